@@ -235,6 +235,74 @@ int32_t s2s_op_attention(void* stream, const void* q, int64_t q_rs, const void* 
                          int32_t use_mfma, void* vt_scratch_dev);
 
 /* ------------------------------------------------------------------------- *
+ * Rotary positions and the paged key / value cache (operators for serving loops whose sessions differ in length by more than a
+ * slot's max_pos rows would allow for; the engines above keep their per-slot caches).
+ *
+ * Rotary tables: cos_dev / sin_dev f32 [max_pos][rotary_dim / 2], cosine and sine (times any attention factor) of position x frequency,
+ * as for s2s_tts tensors "rope.cos" / "rope.sin"; scaled position ranges are scaled tables (speech-to-speech_amd/paged_kv.py builds them
+ * in 64 bits).  The first rotary_dim channels of a head turn (even, 2 .. head_dim), the others pass.  interleaved = 0: channel i is paired
+ * with i + rotary_dim / 2; 1: channel 2 i with 2 i + 1.  (a, b) -> (a c - b s, b c + a s), each product and sum rounded in f32, the
+ * result rounded once to the row type.
+ *
+ * A page holds page_size positions of every KV head:
+ *   keys    [n_pages][kv_heads][page_size][head_dim]       values  [n_pages][kv_heads][head_dim][page_size]   (transposed)
+ * in the row type (S2S_KV_MODEL), or in 4 bits (S2S_KV_INT4, bf16 rows): 32 channels of one position share a scale and a zero,
+ *   value = zero + scale * (code - 8), scale = f16((max - min) / 15), zero = f16(min + 8 scale), code = clamp(rint((x - zero) / scale) + 8, 0, 15)
+ * (scale 0: code 8; inputs beyond +-32768 are cut there; a group with a NaN or an infinity reads back as NaN).  Keys are quantised as the
+ * row type would have held them: turned, then rounded.
+ *   key codes   [n_pages][kv_heads][page_size][head_dim / 2 bytes]: dword g * (head_dim / 32) + s of a row = channels 32 s + 8 g .. + 7
+ *   value codes [n_pages][kv_heads][head_dim][page_size / 2 bytes]: dword o of a row = positions 8 o .. 8 o + 7 of the page
+ *   element e of a dword's 8 is nibble (e >> 1) + 4 (e & 1)
+ *   k_meta f16 [n_pages][kv_heads][page_size][head_dim / 32][2] {scale, zero};  v_meta f16 [n_pages][kv_heads][head_dim / 32][2][page_size]
+ * head_dim 64, 128 or 256; page_size a power of two, 64 .. 1024; buffers aligned to 16 bytes.  No buffer needs initialising.
+ *
+ * table_dev int32 [B][table_cols]: page numbers of every session in order; a number outside [0, n_pages) is no page: rows for it are not
+ * stored, its positions are not attended to.  A page that is written must belong to one session only; pages that are only read may be shared.
+ * cu_dev int32 [B + 1]: session b's new rows are cu[b] .. cu[b + 1] - 1 of the row buffers (T rows); NULL: one row per session (T = B).
+ * max_new: host-side bound of every session's new rows; max_kv: of every kv_len.  Buffers are read with row strides *_rs in elements, the
+ * heads of a row lie next to each other.  Rows at and behind cu[B] are left as they are. */
+#define S2S_KV_MODEL 0
+#define S2S_KV_INT4 1
+typedef struct s2s_paged_kv {
+    void* k;               /* pages of keys / values: see above */
+    void* v;
+    void* k_meta;          /* f16, S2S_KV_INT4 only (else NULL) */
+    void* v_meta;
+    int32_t n_pages, page_size, kv_heads, head_dim;
+    int32_t kind;          /* S2S_KV_MODEL or S2S_KV_INT4 */
+    int32_t dtype;         /* row type of q, k, v and o: S2S_F32 or S2S_BF16 (S2S_KV_INT4: S2S_BF16) */
+} s2s_paged_kv;
+
+/* out[r][h][:] = x[r][h][:] turned to positions_dev[r] (int32).  Element (r, h, d) at r * x_rs + h * x_hs + d; out may be x (same strides).
+ * A row whose position is negative is left as it is; a position >= max_pos makes the turned channels NaN.  head_dim <= 1024. */
+int32_t s2s_op_rope(void* stream, const void* x, int64_t x_rs, int64_t x_hs, void* out, int64_t o_rs, int64_t o_hs, const int32_t* positions_dev,
+                    const float* cos_dev, const float* sin_dev, int32_t max_pos, int32_t rows, int32_t heads, int32_t head_dim, int32_t rotary_dim,
+                    int32_t interleaved, int32_t dtype);
+
+/* Appends every session's new rows behind the start_dev[b] (int32, >= 0) positions its pages hold: the keys turned to their positions, the values as
+ * they are.  cos_dev NULL: keys are stored as they come (rotary_dim ignored).  q (optional, H heads) is turned along into q_out (may be q). */
+int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, const void* k, int64_t k_rs, const void* v, int64_t v_rs, const void* q, int64_t q_rs,
+                               void* q_out, int64_t qo_rs, int32_t H, const int32_t* table_dev, int32_t table_cols, const int32_t* start_dev,
+                               const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, const float* cos_dev, const float* sin_dev, int32_t max_pos,
+                               int32_t rotary_dim, int32_t interleaved);
+
+/* Rows back out of the pages, as the values the cache stands for: position start[b] + i of session b -> row cu[b] + i of k_out / v_out
+ * (row type, row stride o_rs; either may be NULL).  Positions without a page read as zero. */
+int32_t s2s_op_kv_read_paged(void* stream, const s2s_paged_kv* kv, const int32_t* table_dev, int32_t table_cols, const int32_t* start_dev,
+                             const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, void* k_out, void* v_out, int64_t o_rs);
+
+/* o = softmax(scale q k^T) v over the pages, H query heads in H / kv_heads neighbours per KV head.  kv_len_dev int32 [B]: positions in the cache,
+ * the new rows' own among them.  causal: new row i of n sees the positions below kv_len - n + i + 1, window > 0 (causal only): the last
+ * `window` of those.  A row that sees nothing is zero.  Pages may hold anything (NaN too) at positions at and behind kv_len; positions below it that
+ * some row of the call sees hold numbers.  Scores, softmax and sums are f32.
+ * ws_dev: s2s_op_attn_paged_ws(...) bytes (0: none needed), overwritten; calls that may run at the same time need one each. */
+int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const void* q, int64_t q_rs, void* o, int64_t o_rs, int32_t H, const int32_t* table_dev,
+                          int32_t table_cols, const int32_t* kv_len_dev, const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, int32_t max_kv,
+                          float scale, int32_t causal, int32_t window, void* ws_dev, int64_t ws_bytes);
+/* bytes of workspace for these sizes, or a negative error code */
+int64_t s2s_op_attn_paged_ws(const s2s_paged_kv* kv, int32_t H, int32_t B, int32_t T, int32_t max_new, int32_t max_kv, int32_t causal, int32_t window);
+
+/* ------------------------------------------------------------------------- *
  * Whisper (encoder + greedy decoder) for one batch of sessions.
  *   Replaces model.get_encoder()(feats), model.detect_language(encoder_outputs) and
  *   model.generate(feats, max_new_tokens, num_beams=1, return_timestamps=False, task, language)

@@ -1,0 +1,520 @@
+// Attention over the paged key / value cache: softmax(scale q k^T) v for ragged new rows of every session (layout: paged.h).
+//
+// One tile of TK positions, per wave, with the scores TRANSPOSED so that a lane keeps one query row (column) for good:
+//   S^T [16 positions][16 rows] = K Q^T       A = key rows from the page, B = query rows held in registers
+//   P^T = exp2(S^T * scale * log2 e - m)      running maximum m and sum l per column: two shuffles per tile, nothing through LDS
+//   O^T [16 channels][16 rows] += V^T P^T     A = value rows of the transposed page, B = P^T straight from the registers S^T was in
+// The C layout of a 16 x 16 product puts rows 4 g + r (g = lane / 16) into lane g's registers, the B layout wants 8 neighbours per lane: the key
+// row that score tile (u, t) reads at index m is chosen as position (m / 4) 8 U + 8 u + 4 t + m % 4, and lane g holds the positions 8 U g + 8 u .. + 7
+// - the 8 neighbours whose values it loads as one octet.  Grouped heads: a column is a (new row, head of the KV head's group) pair, so the group
+// shares one pass over the pages.
+#include "paged.h"
+
+#include <algorithm>
+
+namespace s2s {
+
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
+
+struct PagedAttn {
+    PagedRows r;
+    const void *kc, *vc;
+    const _Float16 *km, *vm;
+    const void* q; long q_rs;
+    void* o; long o_rs;
+    bool q_vec, o_vec;            // rows allow 16-byte reads / 4-element writes
+    const int* kv_len;
+    int H, G;                     // query heads, query heads per KV head
+    int max_kv, causal, window;
+    float scale_log2e;
+    int n_splits, chunk;          // positions per split (multiple of 64)
+    int q_tiles;
+    float *po, *plse;             // n_splits > 1: [split][T][H][D], [split][T][H] (log2 of the sum of exp2)
+};
+
+template <int KIND> struct KvT;
+template <> struct KvT<KV_F32> {
+    typedef float row_t;
+    typedef f32x8_t frag_t;
+    static constexpr int TK = 32;
+};
+template <> struct KvT<KV_BF16> {
+    typedef __hip_bfloat16 row_t;
+    typedef bf16x8_t frag_t;
+    static constexpr int TK = 64;
+};
+template <> struct KvT<KV_INT4> {  // codes become float16: (code - 8) scale + zero is rounded once, to 11 bits
+    typedef __hip_bfloat16 row_t;
+    typedef f16x8_t frag_t;
+    static constexpr int TK = 64;
+};
+
+// 32-deep step of a 16 x 16 product: lane l holds row l % 16, elements 8 (l / 16) .. + 7 of both operands (f32: eight 4-deep products; both operands
+// deal their elements out alike, so the order within the 32 does not matter)
+__device__ __forceinline__ f32x4_t mma(const bf16x8_t& a, const bf16x8_t& b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4_t mma(const f16x8_t& a, const f16x8_t& b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4_t mma(const f32x8_t& a, const f32x8_t& b, f32x4_t c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+// octet with the elements outside [lo, hi) set to zero (positions nobody attends to may hold NaN, and 0 x NaN is NaN)
+template <typename F> __device__ __forceinline__ void keep_range(F& f, int first, int lo, int hi) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (first + e < lo || first + e >= hi) f[e] = 0;
+}
+
+// where the columns of a tile of query rows stand
+struct Span {
+    int row0, n;                  // rows of the session
+    int len, past;                // positions that count, and before the new rows' own (negative: the first rows see nothing)
+    int lo, hi;                   // positions some row of the tile sees: [lo, hi)
+    int lo_all, hi_all;           // positions every row sees
+};
+__device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, int nvr, Span& s) {
+    session_rows(p.r, b, s.row0, s.n);
+    if (s.n <= 0 || s.row0 >= p.r.T || vr0 >= s.n * p.G) return false;
+    s.len = max(0, min(p.kv_len[b], p.max_kv));
+    s.past = s.len - s.n;
+    const int t0 = vr0 / p.G, t1 = min(vr0 + nvr, s.n * p.G) - 1;
+    const int t_last = t1 / p.G;
+    s.hi = p.causal ? max(0, min(s.len, s.past + t_last + 1)) : s.len;
+    s.hi_all = p.causal ? max(0, min(s.len, s.past + t0 + 1)) : s.len;
+    s.lo = p.window > 0 ? max(0, s.past + t0 + 1 - p.window) : 0;
+    s.lo_all = p.window > 0 ? max(0, s.past + t_last + 1 - p.window) : 0;
+    return true;
+}
+
+// 4 octets of a query row per 128 channels in the operand's type.  4-bit caches: float16 after dividing the row by a power of two (exact), so that its
+// largest value lies in [1, 2); `mul` gives it back.
+template <int KIND, int D>
+__device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row, bool valid, bool vec, int g, typename KvT<KIND>::frag_t (&q)[D / 32],
+                                           float& mul) {
+    mul = 1.f;
+    typedef typename KvT<KIND>::row_t T;
+    typedef typename KvT<KIND == KV_INT4 ? KV_BF16 : KIND>::frag_t raw_t;
+    float x[D / 32][8];
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+        raw_t w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = 0;
+        if (valid) {
+            if (vec) {
+                w = *reinterpret_cast<const raw_t*>(row + s * 32 + g * 8);
+            } else {
+                T one[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) one[e] = row[s * 32 + g * 8 + e];
+                __builtin_memcpy(&w, one, sizeof(one));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = (float)w[e];
+    }
+    if constexpr (KIND == KV_INT4) {
+        float m = 0.f;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[s][e]));
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const int ex = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
+        mul = ldexpf(1.f, ex);
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)ldexpf(x[s][e], -ex);
+    } else if constexpr (KIND == KV_BF16) {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = (__bf16)x[s][e];
+    } else {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[s][e] = x[s][e];
+    }
+}
+
+// (code - 8) scale + zero of an octet
+__device__ __forceinline__ f16x8_t dequant(unsigned w, f16x2_t s0, f16x2_t s1, f16x2_t s2, f16x2_t s3, f16x2_t z0, f16x2_t z1, f16x2_t z2, f16x2_t z3) {
+    f16x2_t c[4];
+    codes_to_f16(w, c);
+    const f16x2_t a = __builtin_elementwise_fma(c[0], s0, z0), b = __builtin_elementwise_fma(c[1], s1, z1);
+    const f16x2_t d = __builtin_elementwise_fma(c[2], s2, z2), e = __builtin_elementwise_fma(c[3], s3, z3);
+    return f16x8_t{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+__device__ __forceinline__ f16x8_t dequant_key(unsigned w, unsigned meta) {
+    const f16x2_t m = __builtin_bit_cast(f16x2_t, meta);
+    const f16x2_t s = {m[0], m[0]}, z = {m[1], m[1]};
+    return dequant(w, s, s, s, s, z, z, z, z);
+}
+__device__ __forceinline__ f16x8_t dequant_val(unsigned w, const f16x8_t& s, const f16x8_t& z) {
+    return dequant(w, f16x2_t{s[0], s[1]}, f16x2_t{s[2], s[3]}, f16x2_t{s[4], s[5]}, f16x2_t{s[6], s[7]}, f16x2_t{z[0], z[1]}, f16x2_t{z[2], z[3]}, f16x2_t{z[4], z[5]},
+                   f16x2_t{z[6], z[7]});
+}
+
+// One tile's keys / values as a wave holds them: what was loaded (raw), and the operand of one product from it.
+template <int KIND, int D> struct KeyTile {       // bf16, f32: octets of the U x 2 rows this lane stands for
+    static constexpr int U = KvT<KIND>::TK / 32;
+    typename KvT<KIND>::frag_t f[U][2][D / 32];
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
+        typedef typename KvT<KIND>::row_t T;
+        const T* base = (const T*)p.kc + ((head << p.r.ps_log2) + at + (l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s = 0; s < D / 32; ++s) f[u][t][s] = *reinterpret_cast<const typename KvT<KIND>::frag_t*>(base + (u * 8 + t * 4) * D + s * 32);
+    }
+    __device__ __forceinline__ typename KvT<KIND>::frag_t get(int u, int t, int s) const { return f[u][t][s]; }
+};
+template <int KIND, int D> struct ValTile {
+    static constexpr int U = KvT<KIND>::TK / 32;
+    typename KvT<KIND>::frag_t f[D / 16][U];
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
+        typedef typename KvT<KIND>::row_t T;
+        const T* base = (const T*)p.vc + ((head * D + l15) << p.r.ps_log2) + at + g * 8 * U;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+            for (int u = 0; u < U; ++u) f[d][u] = *reinterpret_cast<const typename KvT<KIND>::frag_t*>(base + ((long)d * 16 << p.r.ps_log2) + u * 8);
+    }
+    __device__ __forceinline__ typename KvT<KIND>::frag_t get(int d, int u) const { return f[d][u]; }
+};
+template <int D> struct KeyTile<KV_INT4, D> {
+    static constexpr int U = 2, NS = D / 32;
+    unsigned w[U][2][NS], m[U][2][NS];
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
+        const long row = (head << p.r.ps_log2) + at + (l15 >> 2) * 8 * U + (l15 & 3);
+        const unsigned* base = (const unsigned*)p.kc + row * (D / 8) + g * NS;
+        const unsigned* meta = (const unsigned*)p.km + row * NS;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                __builtin_memcpy(w[u][t], __builtin_assume_aligned(base + (u * 8 + t * 4) * (D / 8), NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+                __builtin_memcpy(m[u][t], __builtin_assume_aligned(meta + (u * 8 + t * 4) * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+            }
+    }
+    __device__ __forceinline__ f16x8_t get(int u, int t, int s) const { return dequant_key(w[u][t][s], m[u][t][s]); }
+};
+template <int D> struct ValTile<KV_INT4, D> {
+    static constexpr int U = 2;
+    unsigned w[D / 16][U];
+    f16x8_t s[D / 32][U], z[D / 32][U];
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
+        const unsigned* base = (const unsigned*)p.vc + ((head * D + l15) << (p.r.ps_log2 - 3)) + (at >> 3) + g * U;
+        const _Float16* meta = p.vm + ((head * (D / 32) * 2) << p.r.ps_log2) + at + g * 8 * U;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) __builtin_memcpy(w[d], __builtin_assume_aligned(base + ((long)d * 16 << (p.r.ps_log2 - 3)), U * 4), U * 4);
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                s[k][u] = *reinterpret_cast<const f16x8_t*>(meta + ((long)(2 * k) << p.r.ps_log2) + u * 8);
+                z[k][u] = *reinterpret_cast<const f16x8_t*>(meta + ((long)(2 * k + 1) << p.r.ps_log2) + u * 8);
+            }
+    }
+    __device__ __forceinline__ f16x8_t get(int d, int u) const { return dequant_val(w[d][u], s[d >> 1][u], z[d >> 1][u]); }
+};
+
+// 4 neighbouring channels of an output row
+__device__ __forceinline__ void store4(float* o, const f32x4_t& v, bool vec) {
+    if (vec) {
+        *reinterpret_cast<f32x4_t*>(o) = v;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = v[r];
+}
+__device__ __forceinline__ void store4(__hip_bfloat16* o, const f32x4_t& v, bool vec) {
+    const u32x2_t w = {pack_bf16x2_hw(v[0], v[1]), pack_bf16x2_hw(v[2], v[3])};
+    if (vec) {
+        *reinterpret_cast<u32x2_t*>(o) = w;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) reinterpret_cast<unsigned short*>(o)[r] = (unsigned short)(w[r >> 1] >> (16 * (r & 1)));
+}
+
+// P^T octet as product operand(s).  bf16: a second operand holds what the first rounding left (p = hi + lo to 16 bits), where the products are not
+// what bounds the kernel.
+__device__ __forceinline__ void probs(const float (&x)[8], f32x8_t& hi) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = x[e];
+}
+__device__ __forceinline__ void probs(const float (&x)[8], f16x8_t& hi) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = (_Float16)x[e];
+}
+__device__ __forceinline__ void probs(const float (&x)[8], bf16x8_t& hi) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) hi[e] = (__bf16)x[e];
+}
+
+// ---- few rows per session: every wave streams its own tiles from memory into registers -----------------------------------------------------
+// grid (q_tiles * n_splits, Hkv, B), 4 waves; wave w takes the split's tiles w, w + 4, ...; the four partial softmaxes meet in LDS at the end.  Bound
+// by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
+// the next values behind this tile's products, so both are in flight while the other is used.
+template <int KIND, int D>
+__global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
+    typedef typename KvT<KIND>::row_t T;
+    typedef typename KvT<KIND>::frag_t frag_t;
+    constexpr int TK = KvT<KIND>::TK, U = TK / 32, NS = D / 32, ND = D / 16;
+    __shared__ float so[2][16][D + 4];
+    __shared__ float sm[4][16], sl[4][16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
+    Span sp;
+    if (!tile_span(p, b, vr0, 16, sp)) return;
+    const int vr = vr0 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
+    const bool valid = vr < sp.n * p.G;
+    const int c_hi = !valid ? 0 : p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
+    const int c_lo = p.window > 0 ? sp.past + t + 1 - p.window : 0;
+    const int k0 = (sp.lo & ~63) + split * p.chunk, k1 = min(sp.hi, k0 + p.chunk);
+
+    frag_t q[NS];
+    float sc;
+    load_query<KIND, D>((const T*)p.q + (sp.row0 + t) * p.q_rs + (long)h * D, valid, p.q_vec, g, q, sc);
+    sc *= p.scale_log2e;
+
+    f32x4_t acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    int kb = k0 + wave * TK;
+    if (kb < k1) {
+        KeyTile<KIND, D> kt;
+        ValTile<KIND, D> vt;
+        const int ps_mask = (1 << p.r.ps_log2) - 1;
+        int page = page_of(p.r, b, kb);
+        {
+            const long head = (long)max(page, 0) * p.r.Hkv + hk;
+            kt.load(p, head, kb & ps_mask, l15, g);
+            vt.load(p, head, kb & ps_mask, l15, g);
+        }
+        for (; kb < k1; kb += 4 * TK) {
+            const int nb = kb + 4 * TK;
+            const int next = nb < k1 ? page_of(p.r, b, nb) : -1;
+            const long nhead = (long)max(next, 0) * p.r.Hkv + hk;
+            const int nat = nb < k1 ? nb & ps_mask : 0;
+            f32x4_t s[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    s[u][tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) s[u][tt] = mma(kt.get(u, tt, k), q[k], s[u][tt]);
+                }
+            if (nb < k1) kt.load(p, nhead, nat, l15, g);
+            if (page >= 0) {
+                const bool edge = kb < sp.lo_all || kb + TK > sp.hi_all;
+                const int pos = kb + g * 8 * U;
+                float x[U][8], mx = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[u][e] = s[u][e >> 2][e & 3] * sc;
+                        if (edge && (pos + u * 8 + e < c_lo || pos + u * 8 + e >= c_hi)) x[u][e] = -INFINITY;
+                        mx = fmaxf(mx, x[u][e]);
+                    }
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m, mx);
+                const float ms = mn == -INFINITY ? 0.f : mn;
+                if (__any(mn > m)) {
+                    const float a = __builtin_amdgcn_exp2f(m - ms);
+                    l *= a;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) acc[d] *= a;
+                }
+                m = mn;
+                frag_t ph[U];
+                bf16x8_t pl[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - ms);
+                        l += x[u][e];
+                    }
+                    probs(x[u], ph[u]);
+                    if constexpr (KIND == KV_BF16) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[u][e] -= (float)ph[u][e];
+                        probs(x[u], pl[u]);
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        frag_t v = vt.get(d, u);
+                        if (edge) keep_range(v, pos + u * 8, sp.lo, sp.hi);
+                        acc[d] = mma(v, ph[u], acc[d]);
+                        if constexpr (KIND == KV_BF16) acc[d] = mma(v, pl[u], acc[d]);
+                    }
+            }
+            if (nb < k1) vt.load(p, nhead, nat, l15, g);
+            page = next;
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // four partial softmaxes of the same 16 columns -> one: common maximum first, then waves 2, 3 onto 0, 1, then 1 onto 0
+    if (g == 0) {
+        sm[wave][l15] = m;
+        sl[wave][l15] = l;
+    }
+    __syncthreads();
+    float M = fmaxf(fmaxf(sm[0][l15], sm[1][l15]), fmaxf(sm[2][l15], sm[3][l15]));
+    const float Ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += sl[w][l15] * __builtin_amdgcn_exp2f(sm[w][l15] - Ms);
+    const float mine = __builtin_amdgcn_exp2f(m - Ms);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] *= mine;
+#pragma unroll
+    for (int half = 2; half >= 1; half >>= 1) {
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(&so[wave - half][l15][d * 16 + g * 4]) = acc[d];
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[d] += *reinterpret_cast<const f32x4_t*>(&so[wave][l15][d * 16 + g * 4]);
+        }
+        __syncthreads();
+    }
+    if (wave != 0 || !valid) return;
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const long row = sp.row0 + t;
+    if (p.n_splits == 1) {
+        T* o = (T*)p.o + row * p.o_rs + (long)h * D + g * 4;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) store4(o + d * 16, L == 0.f ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc[d] * inv, p.o_vec);
+    } else {
+        const long at = ((long)split * p.r.T + row) * p.H + h;
+        if (g == 0) p.plse[at] = L == 0.f ? -INFINITY : M + __builtin_amdgcn_logf(L);
+        if (L == 0.f) return;      // the join reads no row of weight 0
+#pragma unroll
+        for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(p.po + at * D + d * 16 + g * 4) = acc[d] * inv;
+    }
+}
+
+// ---- the splits' partial results of one (row, head) -> its output: a wave each, in split order -----------------------------------------------
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn p) {
+    constexpr int E = D / 64;
+    const int lane = threadIdx.x & 63;
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long)p.r.T * p.H;
+    if (i >= n) return;
+    const int row = (int)(i / p.H), h = (int)(i - (long)row * p.H);
+    if (p.r.cu && (row < p.r.cu[0] || row >= p.r.cu[p.r.B])) return;
+    float M = -INFINITY;
+    for (int s = lane; s < p.n_splits; s += 64) M = fmaxf(M, p.plse[s * n + i]);
+    M = wave_max(M);
+    float acc[E], L = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    const float Ms = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+    for (int s = 0; s < p.n_splits; ++s) {
+        const float lse = p.plse[s * n + i];
+        if (lse == -INFINITY) continue;     // nothing was written for it
+        const float w = __builtin_amdgcn_exp2f(lse - Ms);
+        L += w;
+        const float* src = p.po + (s * n + i) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    T* o = (T*)p.o + row * p.o_rs + (long)h * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) Elem<T>::st(o + e, L == 0.f ? 0.f : acc[e] * inv);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------------------
+struct PagedPlan {
+    int n_splits, chunk, q_tiles;
+};
+// How many query tiles and splits: enough workgroups for two on every CU, no split shorter than 256 positions (a tile per wave).
+static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, int max_kv, int causal, int window) {
+    PagedPlan pl;
+    const int G = H / kv->kv_heads;
+    pl.q_tiles = cdiv((long)max_new * G, 16);
+    const long span = std::min<long>(max_kv, causal && window > 0 ? (long)window + cdiv(15, G) + 1 + 63 : max_kv) + 63;
+    const long groups = (long)B * kv->kv_heads * pl.q_tiles;
+    const long want = std::max<long>(1, 1024 / std::max<long>(1, groups));
+    pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
+    pl.n_splits = std::max(1, cdiv(span, pl.chunk));
+    if (pl.n_splits == 1) pl.chunk = 1 << 30;
+    return pl;
+}
+
+template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
+    attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
+    if (p.n_splits > 1) attn_paged_join_kernel<T, D><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
+}
+
+}  // namespace s2s
+
+using namespace s2s;
+
+static int attn_paged_sizes(const s2s_paged_kv* kv, int H, int B, int T, int max_new, int max_kv, int causal, int window) {
+    if (const int rc = paged_check(kv, "attn_paged")) return rc;
+    S2S_REQUIRE(H >= 1 && H <= 4096 && H % kv->kv_heads == 0, "attn_paged: %d query heads over %d KV heads", H, kv->kv_heads);
+    S2S_REQUIRE(B >= 0 && B <= 65535 && T >= 0 && max_new >= 1, "attn_paged: B=%d T=%d max_new=%d", B, T, max_new);
+    S2S_REQUIRE(max_kv >= 0 && max_kv <= 1 << 30, "attn_paged: max_kv=%d", max_kv);
+    S2S_REQUIRE(window >= 0 && (window == 0 || causal), "attn_paged: a window (%d) needs the causal mask", window);
+    return S2S_OK;
+}
+
+extern "C" int64_t s2s_op_attn_paged_ws(const s2s_paged_kv* kv, int32_t H, int32_t B, int32_t T, int32_t max_new, int32_t max_kv, int32_t causal, int32_t window) {
+    if (const int rc = attn_paged_sizes(kv, H, B, T, max_new, max_kv, causal, window)) return rc;
+    if (B == 0 || T == 0) return 0;
+    const PagedPlan pl = paged_plan(kv, H, B, std::min(max_new, T), max_kv, causal, window);
+    return pl.n_splits == 1 ? 0 : (int64_t)pl.n_splits * T * H * (kv->head_dim + 1) * 4;
+}
+
+extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const void* q, int64_t q_rs, void* o, int64_t o_rs, int32_t H, const int32_t* table_dev,
+                                     int32_t table_cols, const int32_t* kv_len_dev, const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, int32_t max_kv,
+                                     float scale, int32_t causal, int32_t window, void* ws_dev, int64_t ws_bytes) {
+    int rc = attn_paged_sizes(kv, H, B, T, max_new, max_kv, causal, window);
+    if (rc) return rc;
+    PagedAttn p{};
+    if ((rc = paged_rows(p.r, kv, table_dev, table_cols, cu_dev, B, T, max_new, "attn_paged"))) return rc;
+    S2S_REQUIRE(max_kv <= table_cols * kv->page_size, "attn_paged: max_kv=%d of %d pages per session", max_kv, table_cols);
+    if (B == 0 || T == 0) return S2S_OK;
+    S2S_REQUIRE(q && o && kv_len_dev, "attn_paged: null buffer");
+    const PagedPlan pl = paged_plan(kv, H, B, p.r.max_new, max_kv, causal, window);
+    const int64_t need = pl.n_splits == 1 ? 0 : (int64_t)pl.n_splits * T * H * (kv->head_dim + 1) * 4;
+    S2S_REQUIRE(need == 0 || (ws_dev && ws_bytes >= need && !((uintptr_t)ws_dev & 15)), "attn_paged: workspace of %lld bytes, 16-byte aligned, needed (got %lld)",
+                (long long)need, (long long)ws_bytes);
+    p.kc = kv->k; p.vc = kv->v; p.km = (const _Float16*)kv->k_meta; p.vm = (const _Float16*)kv->v_meta;
+    p.q = q; p.q_rs = q_rs; p.o = o; p.o_rs = o_rs; p.kv_len = kv_len_dev;
+    const int es = kv->dtype == S2S_F32 ? 4 : 2;
+    p.q_vec = !((uintptr_t)q & 15) && (q_rs * es) % 16 == 0;
+    p.o_vec = !((uintptr_t)o & 15) && (o_rs * es) % 16 == 0;
+    p.H = H; p.G = H / kv->kv_heads; p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
+    p.scale_log2e = scale * 1.44269504088896340736f;
+    p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles;
+    p.po = (float*)ws_dev;
+    p.plse = p.po + (int64_t)pl.n_splits * T * H * kv->head_dim;
+    S2S_PAGED_DISPATCH(attn_launch, (hipStream_t)stream, p);
+    S2S_LAUNCH_CHECK();
+    return S2S_OK;
+}

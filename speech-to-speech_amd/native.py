@@ -20,6 +20,7 @@ DEV_HEADER_PATH = os.path.join(REPO_ROOT, "include", "s2s_mi355x_dev.h")
 S2S_F32, S2S_BF16 = 0, 1
 ACT_NONE, ACT_GELU, ACT_SILU, ACT_RELU = 0, 1, 2, 3
 FRONTEND_WHISPER, FRONTEND_PARAKEET = 0, 1
+S2S_KV_MODEL, S2S_KV_INT4 = 0, 1
 
 
 class WhisperConfigStruct(C.Structure):
@@ -46,6 +47,13 @@ class TTSConfigStruct(C.Structure):
                 + [("up_rate", C.c_int32 * 4), ("up_ratio", C.c_int32 * 2)]
                 + [(n, C.c_int32) for n in ("total_upsample", "max_prompt", "max_frames", "max_pos", "max_codec_frames")]
                 + [("eps", C.c_float), ("c_eps", C.c_float), ("dtype", C.c_int32)])
+
+
+class PagedKVStruct(C.Structure):
+    """Mirror of ``s2s_paged_kv``."""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_meta", "v_meta")]
+                + [(n, C.c_int32) for n in ("n_pages", "page_size", "kv_heads", "head_dim", "kind", "dtype")])
 
 
 class NativeError(RuntimeError):
@@ -86,6 +94,11 @@ _SIGNATURES = {
     "s2s_op_conv1d_causal_tm": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
     "s2s_op_attention": [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32,
                          _i32, _i32, _i32, _vp],
+    "s2s_op_rope": [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
+    "s2s_op_kv_append_paged": [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _i32],
+    "s2s_op_kv_read_paged": [_vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _i64],
+    "s2s_op_attn_paged": [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64],
+    "s2s_op_attn_paged_ws": [_vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
     "s2s_whisper_create": [_vp, _i32, C.POINTER(_vp)],
     "s2s_whisper_destroy": [_vp],
     "s2s_whisper_set_tensor": [_vp, C.c_char_p, _vp, _i64],
@@ -156,7 +169,7 @@ _DEV_SIGNATURES = {
 }
 _RESTYPES = {"s2s_last_error": C.c_char_p, "s2s_whisper_workspace_bytes": C.c_int64,
              "s2s_parakeet_workspace_bytes": C.c_int64, "s2s_tts_workspace_bytes": C.c_int64,
-             "s2s_codec_samples": C.c_int64, "s2s_prof_event_overhead_us": C.c_double}
+             "s2s_codec_samples": C.c_int64, "s2s_op_attn_paged_ws": C.c_int64, "s2s_prof_event_overhead_us": C.c_double}
 
 
 def load():

@@ -1,0 +1,245 @@
+"""Rotary positions and the paged key / value cache (operators of ``include/s2s_mi355x.h``).
+
+A serving loop whose sessions differ widely in length keeps their keys and values in PAGES of one pool instead of one ``max_pos``-row slot
+per session: a page holds ``page_size`` positions of every KV head, a session owns a row of page numbers.  The cache is held in the model
+type or in 4 bits (bf16 models; a scale and a zero per 32 channels of a position: 0.31 of the bf16 bytes)::
+
+    cache = PagedKVCache(n_pages=4096, kv_heads=8, head_dim=128, kind="int4", device="cuda:0")
+    cos, sin = rope_tables(128, max_pos=131072, theta=1e6, scaling="yarn", factor=4.0, original=32768, device="cuda:0")
+    # prompts: session b's new rows are cu[b] .. cu[b + 1] - 1 of q / k / v, behind the start[b] positions it has
+    q = cache.append(k, v, table, start, cu, max_new=longest, cos=cos, sin=sin, q=q)
+    o = cache.attend(q, table, kv_len, cu, max_new=longest, max_kv=longest_session)
+    # one token per session: no cu
+    q = cache.append(k, v, table, kv_len, cos=cos, sin=sin, q=q)
+    o = cache.attend(q, table, kv_len + 1, max_kv=longest_session + 1)
+
+Everything is enqueued on torch's current stream of the cache's device and nothing synchronises: ``max_new`` and ``max_kv`` are HOST bounds of
+the device-side lengths (a captured graph replays with other lengths below them).  Sessions longer than the bounds are cut to them.  Tensors
+are containers only; there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import native
+
+KINDS = {"model": native.S2S_KV_MODEL, "int4": native.S2S_KV_INT4}
+GROUP = 32  # channels of a position that share a scale and a zero
+
+
+def _require(cond, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+class _on_device:
+    """Make the tensors' device current for the call (a no-op where it is: the usual case, and cheaper than torch's guard)."""
+
+    def __init__(self, device):
+        _require(device.type == "cuda", f"tensors on {device}: the operators run on a GPU only")
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard:
+            self.guard.__exit__(*exc)
+
+
+def _ints(t, n, device, what):
+    _require(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == device,
+             f"{what}: contiguous int32[{n}] on {device} needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _rows(t, heads, dim, dtype, device, what):
+    """[rows][heads][dim] whose heads lie next to each other (a slice of a fused projection's rows is fine)."""
+    _require(t.dim() == 3 and t.shape[2] == dim and t.dtype == dtype and t.device == device and (heads is None or t.shape[1] == heads),
+             f"{what}: {dtype} [rows][{'heads' if heads is None else heads}][{dim}] on {device} needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == dim)), f"{what}: the heads of a row must lie next to each other")
+
+
+def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 0):
+    """-> (float64 angle per position of every channel pair, factor on cosine and sine).
+
+    ``scaling``: "none"; "linear" (positions divided by ``factor``); "ntk" (theta x factor^(d / (d - 2)): the slowest pair is stretched by
+    ``factor``, the fastest kept); "yarn" (pairs that turn more than 32 times within the ``original`` trained positions are kept, those that
+    turn less than once are divided by ``factor``, a ramp in between; attention factor 0.1 ln(factor) + 1)."""
+    _require(rotary_dim >= 2 and rotary_dim % 2 == 0, f"rotary_dim {rotary_dim} must be even")
+    _require(theta > 1 and factor >= 1, f"theta {theta} and factor {factor} must be above 1")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    if scaling == "ntk":
+        _require(rotary_dim > 2, "ntk scaling needs more than one channel pair")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = theta ** (-2.0 * i / rotary_dim)
+    if scaling in ("none", "ntk"):
+        return freq, 1.0
+    if scaling == "linear":
+        return freq / factor, 1.0
+    _require(scaling == "yarn", f"unknown scaling {scaling!r}")
+    _require(original > 0, "yarn scaling needs the original number of positions")
+
+    def pair_that_turns(times):
+        return rotary_dim * math.log(original / (times * 2 * math.pi)) / (2 * math.log(theta))
+
+    lo = max(math.floor(pair_that_turns(32)), 0)
+    hi = min(math.ceil(pair_that_turns(1)), rotary_dim - 1)
+    ramp = ((i - lo) / max(hi - lo, 0.001)).clamp(0, 1)
+    return freq / factor * ramp + freq * (1 - ramp), 0.1 * math.log(factor) + 1.0
+
+
+def rope_tables(rotary_dim: int, max_pos: int, theta: float = 10000.0, *, scaling: str = "none", factor: float = 1.0, original: int = 0, device="cuda"):
+    """Cosine and sine tables float32 [max_pos][rotary_dim / 2], computed in float64 (the angles of far positions lose all digits in float32)."""
+    freq, m = rope_frequencies(rotary_dim, theta, scaling, factor, original)
+    a = torch.arange(max_pos, dtype=torch.float64)[:, None] * freq[None]
+    return (a.cos() * m).float().to(device), (a.sin() * m).float().to(device)
+
+
+def _check_tables(cos, sin, device):
+    _require(cos is not None and sin is not None and cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
+             and cos.is_contiguous() and sin.is_contiguous() and cos.device == device and sin.device == device,
+             f"cos / sin: contiguous float32 [max_pos][rotary_dim / 2] on {device} needed")
+
+
+def rope(x, positions, cos, sin, *, interleaved: bool = False, out=None):
+    """Turn the first ``2 * cos.shape[1]`` channels of every head of ``x`` [rows][heads][dim] to its row's position -> ``out`` (new, or given, or
+    ``x`` itself).  ``positions`` int32 [rows]: a negative one leaves the row of ``out`` as it is, one behind the table gives NaN."""
+    _require(x.dim() == 3 and (x.numel() == 0 or x.stride(2) == 1), "x: [rows][heads][dim] with neighbouring channels needed")
+    _ints(positions, x.shape[0], x.device, "positions")
+    _check_tables(cos, sin, x.device)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _require(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and (x.numel() == 0 or out.stride(2) == 1), "out must match x")
+    with _on_device(x.device):
+        native.check(native.load().s2s_op_rope(native.stream_handle(), x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                                               positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], x.shape[0], x.shape[1], x.shape[2],
+                                               2 * cos.shape[1], 1 if interleaved else 0, native.dtype_code(x.dtype)), "s2s_op_rope")
+    return out
+
+
+class PagedKVCache:
+    """A pool of pages for the keys and values of ONE layer, and the operators on it.  ``k`` / ``v`` (and ``k_meta`` / ``v_meta`` of a 4-bit cache) are
+    the tensors themselves, in the layout of ``s2s_paged_kv``."""
+
+    def __init__(self, n_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64, kind: str = "model", dtype=torch.bfloat16, device="cuda"):
+        _require(kind in KINDS, f"unknown cache kind {kind!r} ({', '.join(KINDS)})")
+        e = dict(device=device)
+        if kind == "model":
+            self._bind(torch.empty(n_pages, kv_heads, page_size, head_dim, dtype=dtype, **e), torch.empty(n_pages, kv_heads, head_dim, page_size, dtype=dtype, **e), None, None)
+        else:
+            _require(dtype == torch.bfloat16, "a 4-bit cache takes bfloat16 rows")
+            g = head_dim // GROUP
+            self._bind(torch.empty(n_pages, kv_heads, page_size, head_dim // 2, dtype=torch.uint8, **e), torch.empty(n_pages, kv_heads, head_dim, page_size // 2, dtype=torch.uint8, **e),
+                       torch.empty(n_pages, kv_heads, page_size, g, 2, dtype=torch.float16, **e), torch.empty(n_pages, kv_heads, g, 2, page_size, dtype=torch.float16, **e))
+
+    @classmethod
+    def adopt(cls, k, v, k_meta=None, v_meta=None) -> "PagedKVCache":
+        """A cache over tensors the caller has (kept by reference): the shapes give pages, heads, sizes and kind."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_meta, v_meta)
+        return self
+
+    def _bind(self, k, v, k_meta, v_meta) -> None:
+        _require(k.dim() == 4 and v.dim() == 4 and k.dtype == v.dtype and k.device == v.device and k.is_contiguous() and v.is_contiguous(),
+                 "pages: contiguous 4-d tensors of one type on one device needed")
+        _require((k_meta is None) == (v_meta is None), "k_meta and v_meta go together")
+        n, h, ps, d = k.shape
+        if k_meta is None:
+            self.kind, self.dtype = "model", k.dtype
+            _require(v.shape == (n, h, d, ps), f"values: {(n, h, d, ps)} needed, got {tuple(v.shape)}")
+        else:
+            self.kind, self.dtype, d = "int4", torch.bfloat16, 2 * d
+            _require(k.dtype == torch.uint8 and v.shape == (n, h, d, ps // 2), "4-bit pages: uint8 [pages][heads][page_size][dim / 2] and [pages][heads][dim][page_size / 2]")
+            _require(k_meta.dtype == v_meta.dtype == torch.float16 and k_meta.shape == (n, h, ps, d // GROUP, 2) and v_meta.shape == (n, h, d // GROUP, 2, ps)
+                     and k_meta.is_contiguous() and v_meta.is_contiguous() and k_meta.device == v_meta.device == k.device, "k_meta / v_meta do not match the pages")
+        self.k, self.v, self.k_meta, self.v_meta = k, v, k_meta, v_meta
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, ps, d, k.device
+        self._kv = native.PagedKVStruct(native.ptr(k), native.ptr(v), native.ptr(k_meta), native.ptr(v_meta), n, ps, h, d, KINDS[self.kind], native.dtype_code(self.dtype))
+        self._ref = C.byref(self._kv)
+
+    def _sessions(self, table, lens, cu, rows, max_new, what):
+        _require(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.device == self.device, f"table: contiguous int32 [sessions][pages] on {self.device} needed")
+        b = table.shape[0]
+        _ints(lens, b, self.device, what)
+        if cu is None:
+            _require(rows == b and max_new in (None, 1), f"without cu there is one row per session ({rows} rows, {b} sessions)")
+            return b, 1
+        _ints(cu, b + 1, self.device, "cu")
+        return b, max(1, rows if max_new is None else max_new)
+
+    def append(self, k, v, table, start, cu=None, *, max_new=None, cos=None, sin=None, interleaved: bool = False, q=None, q_out=None):
+        """Store every session's new rows behind the ``start`` positions its pages hold, keys turned to their positions (``cos`` / ``sin`` None: as they come).
+        ``q`` is turned along -> ``q_out`` (new, or given, or ``q`` itself), which is returned."""
+        _rows(k, self.kv_heads, self.head_dim, self.dtype, self.device, "k")
+        _rows(v, self.kv_heads, self.head_dim, self.dtype, self.device, "v")
+        T = k.shape[0]
+        b, max_new = self._sessions(table, start, cu, T, max_new, "start")
+        _require(v.shape[0] == T and (q is None or q.shape[0] == T), "k, v and q need the same rows")
+        H = 0
+        if cos is not None or sin is not None:
+            _check_tables(cos, sin, self.device)
+        if q is not None:
+            _require(cos is not None, "queries are turned: cos / sin needed")
+            _rows(q, None, self.head_dim, self.dtype, self.device, "q")
+            H = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            _rows(q_out, H, self.head_dim, self.dtype, self.device, "q_out")
+            _require(q_out.shape[0] == T, "q_out needs q's rows")
+        with _on_device(self.device):
+            native.check(native.load().s2s_op_kv_append_paged(
+                native.stream_handle(), self._ref, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), native.ptr(q), q.stride(0) if H else 0, native.ptr(q_out) if H else 0,
+                q_out.stride(0) if H else 0, H, table.data_ptr(), table.shape[1], start.data_ptr(), native.ptr(cu), b, T, max_new, native.ptr(cos), native.ptr(sin),
+                cos.shape[0] if cos is not None else 0, 2 * cos.shape[1] if cos is not None else 0, 1 if interleaved else 0), "s2s_op_kv_append_paged")
+        return q_out if H else None
+
+    def read(self, table, start, cu=None, rows=None, *, max_new=None):
+        """Positions ``start[b] + i`` of every session, back as rows (keys, values) [rows][kv_heads][head_dim] of the model type: what the cache stands for.
+        ``rows`` = cu[-1] where ``cu`` is given."""
+        if rows is None:
+            _require(cu is None, "rows: how many rows cu counts")
+            rows = table.shape[0]
+        b, max_new = self._sessions(table, start, cu, rows, max_new, "start")
+        out = torch.empty(2, rows, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.device)
+        with _on_device(self.device):
+            native.check(native.load().s2s_op_kv_read_paged(native.stream_handle(), self._ref, table.data_ptr(), table.shape[1], start.data_ptr(), native.ptr(cu), b, rows, max_new,
+                                                            out[0].data_ptr(), out[1].data_ptr(), self.kv_heads * self.head_dim), "s2s_op_kv_read_paged")
+        return out[0], out[1]
+
+    def workspace_bytes(self, heads: int, sessions: int, rows: int, *, max_new: int = 1, max_kv: int, causal: bool = True, window: int = 0) -> int:
+        """Bytes ``attend`` needs beside its buffers for these sizes."""
+        n = native.load().s2s_op_attn_paged_ws(self._ref, heads, sessions, rows, max_new, max_kv, 1 if causal else 0, window)
+        if n < 0:
+            native.check(int(n), "s2s_op_attn_paged_ws")
+        return int(n)
+
+    def attend(self, q, table, kv_len, cu=None, *, max_new=None, max_kv=None, scale=None, causal: bool = True, window: int = 0, out=None, workspace=None):
+        """softmax(scale q k^T) v over the first ``kv_len[b]`` positions of every session (the new rows' own among them) -> ``out`` (new, or given).
+        ``q`` [rows][heads][head_dim], heads a multiple of ``kv_heads``; ``scale`` None: head_dim ** -0.5.  causal: new row i of n sees the positions
+        below kv_len - n + i + 1, ``window`` > 0: the last ``window`` of those.  A row that sees nothing is zero.  ``workspace``: uint8 tensor of
+        ``workspace_bytes`` (None: taken from torch's allocator; one given to calls on several streams at once would be overwritten)."""
+        _rows(q, None, self.head_dim, self.dtype, self.device, "q")
+        T, H = q.shape[0], q.shape[1]
+        b, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
+        if max_kv is None:
+            max_kv = table.shape[1] * self.page_size
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _rows(out, H, self.head_dim, self.dtype, self.device, "out")
+        _require(out.shape[0] == T, "out needs q's rows")
+        lib, c = native.load(), 1 if causal else 0
+        with _on_device(self.device):
+            need = lib.s2s_op_attn_paged_ws(self._ref, H, b, T, max_new, max_kv, c, window)
+            if need < 0:
+                native.check(int(need), "s2s_op_attn_paged_ws")
+            if need and workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            native.check(lib.s2s_op_attn_paged(native.stream_handle(), self._ref, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), H, table.data_ptr(), table.shape[1],
+                                               kv_len.data_ptr(), native.ptr(cu), b, T, max_new, max_kv, self.head_dim ** -0.5 if scale is None else scale, c, window,
+                                               native.ptr(workspace), workspace.numel() * workspace.element_size() if workspace is not None else 0), "s2s_op_attn_paged")
+        return out
