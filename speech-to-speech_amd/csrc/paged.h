@@ -57,6 +57,15 @@ __device__ __forceinline__ void session_rows(const PagedRows& r, int b, int& row
     n = min(min(c1, r.T) - row0, r.max_new);
     n = max(n, 0);
 }
+// The same number as a scalar load, not yet looked at: the wait for it falls where page_ok asks.  b and pos must be the same in all lanes (the table is
+// only read by these kernels, so the constant address space holds).
+__device__ __forceinline__ int page_raw(const PagedRows& r, int b, int pos) {
+    const int col = pos >> r.ps_log2;
+    if (pos < 0 || col >= r.cols) return -1;
+    typedef const __attribute__((address_space(4))) int* scalar_t;
+    return ((scalar_t)(uintptr_t)r.table)[(long)b * r.cols + col];
+}
+__device__ __forceinline__ bool page_ok(const PagedRows& r, int pg) { return (unsigned)pg < (unsigned)r.n_pages; }
 __device__ __forceinline__ int page_of(const PagedRows& r, int b, int pos) {
     const int col = pos >> r.ps_log2;
     if (pos < 0 || col >= r.cols) return -1;

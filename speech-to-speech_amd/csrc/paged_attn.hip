@@ -29,6 +29,7 @@ struct PagedAttn {
     float scale_log2e;
     int n_splits, chunk;          // positions per split (multiple of 64)
     int q_tiles;
+    bool tile;                    // attn_paged_tile_kernel (host side)
     float *po, *plse;             // n_splits > 1: [split][T][H][D], [split][T][H] (log2 of the sum of exp2)
 };
 
@@ -264,7 +265,7 @@ __device__ __forceinline__ void probs(const float (&x)[8], bf16x8_t& hi) {
 // by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
 // the next values behind this tile's products, so both are in flight while the other is used.
 template <int KIND, int D>
-__global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND>::frag_t frag_t;
     constexpr int TK = KvT<KIND>::TK, U = TK / 32, NS = D / 32, ND = D / 16;
@@ -295,16 +296,16 @@ __global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
         KeyTile<KIND, D> kt;
         ValTile<KIND, D> vt;
         const int ps_mask = (1 << p.r.ps_log2) - 1;
-        int page = page_of(p.r, b, kb);
+        int page = page_raw(p.r, b, kb), next = kb + 4 * TK < k1 ? page_raw(p.r, b, kb + 4 * TK) : -1;
         {
-            const long head = (long)max(page, 0) * p.r.Hkv + hk;
+            const long head = (long)(page_ok(p.r, page) ? page : 0) * p.r.Hkv + hk;
             kt.load(p, head, kb & ps_mask, l15, g);
             vt.load(p, head, kb & ps_mask, l15, g);
         }
         for (; kb < k1; kb += 4 * TK) {
             const int nb = kb + 4 * TK;
-            const int next = nb < k1 ? page_of(p.r, b, nb) : -1;
-            const long nhead = (long)max(next, 0) * p.r.Hkv + hk;
+            const long nhead = (long)(page_ok(p.r, next) ? next : 0) * p.r.Hkv + hk;
+            const int after = nb + 4 * TK < k1 ? page_raw(p.r, b, nb + 4 * TK) : -1;
             const int nat = nb < k1 ? nb & ps_mask : 0;
             f32x4_t s[U][2];
 #pragma unroll
@@ -316,7 +317,7 @@ __global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
                     for (int k = 0; k < NS; ++k) s[u][tt] = mma(kt.get(u, tt, k), q[k], s[u][tt]);
                 }
             if (nb < k1) kt.load(p, nhead, nat, l15, g);
-            if (page >= 0) {
+            if (page_ok(p.r, page)) {
                 const bool edge = kb < sp.lo_all || kb + TK > sp.hi_all;
                 const int pos = kb + g * 8 * U;
                 float x[U][8], mx = -INFINITY;
@@ -367,6 +368,7 @@ __global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
             }
             if (nb < k1) vt.load(p, nhead, nat, l15, g);
             page = next;
+            next = after;
         }
     }
     l += __shfl_xor(l, 16, 64);
@@ -415,6 +417,254 @@ __global__ __launch_bounds__(256) void attn_paged_step_kernel(PagedAttn p) {
     }
 }
 
+// ---- many rows per session: a workgroup's tile of query rows shares every tile of positions through LDS ----------------------------------------
+// 4 waves x NC x 16 columns.  Tiles of keys and values go from the page into LDS without passing registers (4-bit codes: through registers, as
+// float16), a double buffer and one barrier per tile.  Octets are stored at index o ^ f(row): the 8 lanes that read together hold rows whose f differs,
+// so the 16-byte reads hit every bank once.  Per 32 positions a wave reads 2 KiB x D / 64 of keys and of values for 16 NC columns; at NC = 2 the LDS reads
+// take as long as the products.
+//
+// The running maximum is raised only when a score exceeds it by more than 8 (in log2): P stays below 2^8, sums and products are f32, so nothing is lost,
+// and the usual step needs no cross-lane maximum and no rescaling.
+constexpr float MAX_SLACK = 8.f;
+constexpr float NO_MAX = -3e38f;                  // finite, so that masked scores (-inf) minus it stay -inf
+
+__device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+template <int KIND, int D> struct LdsTile {
+    typedef typename KvT<KIND>::frag_t frag_t;
+    static constexpr int TK = KvT<KIND>::TK, U = TK / 32;
+    static constexpr int EB = KIND == KV_F32 ? 4 : 2;              // bytes per element in LDS
+    static constexpr int K_BYTES = TK * D * EB, BYTES = 2 * K_BYTES;
+    static __device__ __forceinline__ int kf(int key) { return (key & 3) | ((key >> (U == 2 ? 4 : 3)) & 1) << 2; }
+    static __device__ __forceinline__ int vf(int d) { return d & (TK / 8 - 1); }
+    static __device__ __forceinline__ int k_at(int key, int o) { return (key * (D / 8) + (o ^ kf(key))) * 8 * EB; }
+    static __device__ __forceinline__ int v_at(int d, int o) { return K_BYTES + (d * (TK / 8) + (o ^ vf(d))) * 8 * EB; }
+};
+
+// page -> LDS: 16-byte pieces in LDS order, the swizzle in the source address
+template <int KIND, int D>
+__device__ __forceinline__ void tile_dma(const PagedAttn& p, unsigned char* buf, int page, int hk, int at, int wave, int lane) {
+    typedef LdsTile<KIND, D> L;
+    constexpr int PB = L::EB / 2;                                  // pieces per octet
+    constexpr int N = L::K_BYTES / 16 / 256;                       // pieces per thread, keys or values
+    const long head = (long)page * p.r.Hkv + hk;
+    const unsigned char* kb = (const unsigned char*)p.kc + ((head << p.r.ps_log2) + at) * D * L::EB;
+    const unsigned char* vb = (const unsigned char*)p.vc + (((head * D) << p.r.ps_log2) + at) * L::EB;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c0 = (i * 4 + wave) * 64, c = c0 + lane, o = c / PB, half = c % PB;
+        const int key = o / (D / 8), ko = (o % (D / 8)) ^ L::kf(key);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + (long)(key * D + ko * 8) * L::EB + half * 16),
+                                         (__attribute__((address_space(3))) void*)(buf + c0 * 16), 16, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int c0 = (i * 4 + wave) * 64, c = c0 + lane, o = c / PB, half = c % PB;
+        const int d = o / (L::TK / 8), vo = (o % (L::TK / 8)) ^ L::vf(d);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + (((long)d << p.r.ps_log2) + vo * 8) * L::EB + half * 16),
+                                         (__attribute__((address_space(3))) void*)(buf + L::K_BYTES + c0 * 16), 16, 0, 0);
+    }
+}
+// 4-bit page -> registers: D / 32 octets of one key and D / 32 octets of one value channel per thread, with their scales and zeros
+template <int D> struct CodeRegs {
+    static constexpr int NS = D / 32;
+    unsigned kw[NS], km[NS], vw[NS];
+    f16x8_t vs[NS], vz[NS];
+    __device__ __forceinline__ void load(const PagedAttn& p, int page, int hk, int at, int tid) {
+        const long head = (long)page * p.r.Hkv + hk;
+        const int key = tid >> 2, g = tid & 3, d = tid * NS / 8, o = tid * NS % 8;
+        const long row = (head << p.r.ps_log2) + at + key;
+        __builtin_memcpy(kw, __builtin_assume_aligned((const unsigned*)p.kc + row * (D / 8) + g * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+        __builtin_memcpy(km, __builtin_assume_aligned((const unsigned*)p.km + row * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+        __builtin_memcpy(vw, __builtin_assume_aligned((const unsigned*)p.vc + ((head * D + d) << (p.r.ps_log2 - 3)) + (at >> 3) + o, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+        const _Float16* m = p.vm + ((head * NS + d / 32) * 2 << p.r.ps_log2) + at + o * 8;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            vs[j] = *reinterpret_cast<const f16x8_t*>(m + j * 8);
+            vz[j] = *reinterpret_cast<const f16x8_t*>(m + ((long)1 << p.r.ps_log2) + j * 8);
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* buf, int tid) const {
+        typedef LdsTile<KV_INT4, D> L;
+        const int key = tid >> 2, g = tid & 3, d = tid * NS / 8, o = tid * NS % 8;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) *reinterpret_cast<f16x8_t*>(buf + L::k_at(key, 4 * s + g)) = dequant_key(kw[s], km[s]);
+#pragma unroll
+        for (int j = 0; j < NS; ++j) *reinterpret_cast<f16x8_t*>(buf + L::v_at(d, o + j)) = dequant_val(vw[j], vs[j], vz[j]);
+    }
+};
+
+template <int KIND, int D, int NC>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(PagedAttn p) {
+    typedef typename KvT<KIND>::row_t T;
+    typedef typename KvT<KIND>::frag_t frag_t;
+    typedef LdsTile<KIND, D> L;
+    constexpr int TK = L::TK, U = L::U, NS = D / 32, ND = D / 16, RW = NC * 16;
+    __shared__ alignas(16) unsigned char lds[2 * L::BYTES];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+    // workgroups with the same (session, KV head) read the same pages: where the count allows, they go to one XCD (ids round-robin over 8) and meet in
+    // its L2.  Late query tiles see the most positions and come first.
+    const int per = p.q_tiles * p.n_splits, pairs = p.r.B * p.r.Hkv;
+    int pair, w;
+    if (pairs % 8 == 0) {
+        const int j = blockIdx.x >> 3;
+        pair = (j / per) * 8 + (blockIdx.x & 7);
+        w = j % per;
+    } else {
+        pair = blockIdx.x / per;
+        w = blockIdx.x % per;
+    }
+    const int b = pair / p.r.Hkv, hk = pair % p.r.Hkv, split = w % p.n_splits, vr0 = (p.q_tiles - 1 - w / p.n_splits) * 4 * RW;
+    Span sp, sw;
+    if (!tile_span(p, b, vr0, 4 * RW, sp)) return;
+    if (!tile_span(p, b, vr0 + wave * RW, RW, sw)) sw.lo = sw.hi = sw.lo_all = sw.hi_all = 0;      // no rows: help with the tiles only
+    const int nvr = sp.n * p.G;
+    const int k0 = (sp.lo & ~63) + split * p.chunk, k1 = min(sp.hi, k0 + p.chunk);
+
+    frag_t q[NC][NS];
+    float sc[NC], m[NC], l[NC];
+    f32x4_t acc[NC][ND];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int vr = vr0 + wave * RW + c * 16 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
+        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, vr < nvr, p.q_vec, g, q[c], sc[c]);
+        sc[c] *= p.scale_log2e;
+        m[c] = NO_MAX;
+        l[c] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int ps_mask = (1 << p.r.ps_log2) - 1;
+    int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, cur = 0;
+    int next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1;
+    CodeRegs<KIND == KV_INT4 ? D : 32> regs;
+    if constexpr (KIND == KV_INT4) {
+        if (page_ok(p.r, page)) {
+            regs.load(p, page, hk, k0 & ps_mask, tid);
+            regs.store(lds, tid);
+        }
+        if (page_ok(p.r, next)) regs.load(p, next, hk, (k0 + TK) & ps_mask, tid);
+    } else {
+        if (page_ok(p.r, page)) tile_dma<KIND, D>(p, lds, page, hk, k0 & ps_mask, wave, lane);
+    }
+    for (int kb = k0; kb < k1; kb += TK) {
+        __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed
+        __builtin_amdgcn_s_barrier();              // everyone's has, and everyone is done with the other buffer
+        const unsigned char* buf = lds + cur * L::BYTES;
+        unsigned char* other = lds + (cur ^ 1) * L::BYTES;
+        const int after = kb + 2 * TK < k1 ? page_raw(p.r, b, kb + 2 * TK) : -1;
+        if constexpr (KIND == KV_INT4) {
+            if (page_ok(p.r, next)) regs.store(other, tid);
+            if (page_ok(p.r, after)) regs.load(p, after, hk, (kb + 2 * TK) & ps_mask, tid);
+        } else {
+            if (page_ok(p.r, next)) tile_dma<KIND, D>(p, other, next, hk, (kb + TK) & ps_mask, wave, lane);
+        }
+        if (page_ok(p.r, page) && kb < sw.hi && kb + TK > sw.lo) {
+            const bool edge = kb < sw.lo_all || kb + TK > sw.hi_all;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                f32x4_t s[NC][2];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    const int key = (l15 >> 2) * 8 * U + u * 8 + tt * 4 + (l15 & 3);
+#pragma unroll
+                    for (int k = 0; k < NS; ++k) {
+                        const frag_t a = *reinterpret_cast<const frag_t*>(buf + L::k_at(key, 4 * k + g));
+#pragma unroll
+                        for (int c = 0; c < NC; ++c) s[c][tt] = mma(a, q[c][k], s[c][tt]);
+                    }
+                }
+                const int pos = kb + g * 8 * U + u * 8;
+                float x[NC][8];
+                bool raise = false;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    if (edge) {
+                        const int t = (vr0 + wave * RW + c * 16 + l15) / p.G;
+                        const int hi = p.causal ? min(sp.len, sp.past + t + 1) : sp.len, lo = p.window > 0 ? sp.past + t + 1 - p.window : 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (pos + e < lo || pos + e >= hi) s[c][e >> 2][e & 3] = -INFINITY;
+                    }
+                    float mx = NO_MAX;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -m[c]);
+                        mx = fmaxf(mx, x[c][e]);
+                    }
+                    raise |= mx > MAX_SLACK;
+                }
+                if (__any(raise)) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        float mx = m[c];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[c][e >> 2][e & 3] * sc[c]);
+                        mx = max_over_groups(mx);
+                        const float a = __builtin_amdgcn_exp2f(m[c] - mx);
+                        m[c] = mx;
+                        l[c] *= a;
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) acc[c][d] *= a;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -mx);
+                    }
+                }
+                frag_t pr[NC];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
+                        l[c] += x[c][e];
+                    }
+                    probs(x[c], pr[c]);
+                }
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    frag_t v = *reinterpret_cast<const frag_t*>(buf + L::v_at(d * 16 + l15, g * U + u));
+                    if (edge) keep_range(v, pos, sp.lo, sp.hi);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) acc[c][d] = mma(v, pr[c], acc[c][d]);
+                }
+            }
+        }
+        page = next;
+        next = after;
+        cur ^= 1;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int vr = vr0 + wave * RW + c * 16 + l15;
+        l[c] += __shfl_xor(l[c], 16, 64);
+        l[c] += __shfl_xor(l[c], 32, 64);
+        if (vr >= nvr) continue;
+        const int t = vr / p.G, h = hk * p.G + vr % p.G;
+        const float inv = l[c] > 0.f ? 1.f / l[c] : 0.f;
+        const bool none = l[c] == 0.f;
+        const long row = sp.row0 + (long)t;
+        if (p.n_splits == 1) {
+            T* o = (T*)p.o + row * p.o_rs + (long)h * D + g * 4;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) store4(o + d * 16, none ? f32x4_t{0.f, 0.f, 0.f, 0.f} : acc[c][d] * inv, p.o_vec);
+        } else {
+            const long at = ((long)split * p.r.T + row) * p.H + h;
+            if (g == 0) p.plse[at] = none ? -INFINITY : m[c] + __builtin_amdgcn_logf(l[c]);
+            if (none) continue;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(p.po + at * D + d * 16 + g * 4) = acc[c][d] * inv;
+        }
+    }
+}
+
 // ---- the splits' partial results of one (row, head) -> its output: a wave each, in split order -----------------------------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn p) {
@@ -450,13 +700,17 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn p) {
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
 struct PagedPlan {
     int n_splits, chunk, q_tiles;
+    bool tile;                    // attn_paged_tile_kernel
 };
-// How many query tiles and splits: enough workgroups for two on every CU, no split shorter than 256 positions (a tile per wave).
+constexpr int tile_nc(int kind, int D) { return D == 256 && kind != KV_BF16 ? 1 : 2; }     // 256 channels: what the registers hold
+// Which kernel, how many query tiles and splits: enough workgroups for two on every CU, no split shorter than 256 positions (a tile per wave).
 static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, int max_kv, int causal, int window) {
     PagedPlan pl;
     const int G = H / kv->kv_heads;
-    pl.q_tiles = cdiv((long)max_new * G, 16);
-    const long span = std::min<long>(max_kv, causal && window > 0 ? (long)window + cdiv(15, G) + 1 + 63 : max_kv) + 63;
+    pl.tile = (long)max_new * G > 32;
+    const int rows = pl.tile ? 4 * 16 * tile_nc(paged_kind(kv), kv->head_dim) : 16;
+    pl.q_tiles = cdiv((long)max_new * G, rows);
+    const long span = std::min<long>(max_kv, causal && window > 0 ? (long)window + cdiv(rows - 1, G) + 1 + 63 : max_kv) + 63;
     const long groups = (long)B * kv->kv_heads * pl.q_tiles;
     const long want = std::max<long>(1, 1024 / std::max<long>(1, groups));
     pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
@@ -466,7 +720,8 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
 }
 
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
-    attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
+    if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(KIND, D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
+    else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
     if (p.n_splits > 1) attn_paged_join_kernel<T, D><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }
 
@@ -511,7 +766,7 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     p.o_vec = !((uintptr_t)o & 15) && (o_rs * es) % 16 == 0;
     p.H = H; p.G = H / kv->kv_heads; p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles;
+    p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles; p.tile = pl.tile;
     p.po = (float*)ws_dev;
     p.plse = p.po + (int64_t)pl.n_splits * T * H * kv->head_dim;
     S2S_PAGED_DISPATCH(attn_launch, (hipStream_t)stream, p);

@@ -269,7 +269,9 @@ def check_attention(new, kv, Hkv, H, D, ps, kind, dtype, causal=True, window=0, 
             if bb == b:
                 seen[c * ps : (c + 1) * ps] = False
         want, size = R.attend(q[cu[b] : cu[b + 1]].double(), kk, vv, new[b], D**-0.5 if scale is None else scale, causal, window, seen)
-        tol = tolerance(want, size, kind, dtype, float(vv.abs().max()) if kv[b] else 0.0, kv[b], D, few)
+        # the second operand goes with the kernel for at most 32 (row, head) pairs per KV head; above that the weights are one bf16 operand: each is off by
+        # half a step, 2^-8 of itself, and sum p |v| <= vmax
+        tol = tolerance(want, size, kind, dtype, float(vv.abs().max()) if kv[b] else 0.0, kv[b], D, few and max(new) * (H // Hkv) <= 32)
         err = (got[cu[b] : cu[b + 1]] - want).abs()
         assert (err <= tol).all(), (b, float((err / tol).max()), float(err.max()))
     return cache, table
