@@ -37,18 +37,17 @@ template <int KIND> struct KvT;
 template <> struct KvT<KV_F32> {
     typedef float row_t;
     typedef f32x8_t frag_t;
-    static constexpr int TK = 32;
 };
 template <> struct KvT<KV_BF16> {
     typedef __hip_bfloat16 row_t;
     typedef bf16x8_t frag_t;
-    static constexpr int TK = 64;
 };
 template <> struct KvT<KV_INT4> {  // codes become float16: (code - 8) scale + zero is rounded once, to 11 bits
     typedef __hip_bfloat16 row_t;
     typedef f16x8_t frag_t;
-    static constexpr int TK = 64;
 };
+// 32-deep product steps of a tile along the positions: 64 positions, 32 where a tile of 64 would not leave room for a second one in the registers
+constexpr int tile_u(int kind, int D) { return kind == KV_F32 || D == 256 ? 1 : 2; }
 
 // 32-deep step of a 16 x 16 product: lane l holds row l % 16, elements 8 (l / 16) .. + 7 of both operands (f32: eight 4-deep products; both operands
 // deal their elements out alike, so the order within the 32 does not matter)
@@ -60,12 +59,20 @@ __device__ __forceinline__ f32x4_t mma(const f32x8_t& a, const f32x8_t& b, f32x4
     return c;
 }
 
-// octet with the elements outside [lo, hi) set to zero (positions nobody attends to may hold NaN, and 0 x NaN is NaN)
-template <typename F> __device__ __forceinline__ void keep_range(F& f, int first, int lo, int hi) {
+// bits of an octet's elements inside [lo, hi): positions nobody attends to may hold NaN, and 0 x NaN is NaN
+template <typename F> struct OctetBits {
+    static constexpr int N = sizeof(F) / 4;
+    typedef unsigned bits_t __attribute__((ext_vector_type(N)));
+    bits_t w;
+    __device__ __forceinline__ OctetBits(int first, int lo, int hi) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (first + e < lo || first + e >= hi) f[e] = 0;
-}
+        for (int i = 0; i < N; ++i) {
+            if constexpr (N == 8) w[i] = first + i >= lo && first + i < hi ? ~0u : 0u;
+            else w[i] = (first + 2 * i >= lo && first + 2 * i < hi ? 0xffffu : 0u) | (first + 2 * i + 1 >= lo && first + 2 * i + 1 < hi ? 0xffff0000u : 0u);
+        }
+    }
+    __device__ __forceinline__ F keep(const F& f) const { return __builtin_bit_cast(F, __builtin_bit_cast(bits_t, f) & w); }
+};
 
 // where the columns of a tile of query rows stand
 struct Span {
@@ -160,68 +167,97 @@ __device__ __forceinline__ f16x8_t dequant_val(unsigned w, const f16x8_t& s, con
                    f16x2_t{z[6], z[7]});
 }
 
-// One tile's keys / values as a wave holds them: what was loaded (raw), and the operand of one product from it.
+// One tile's keys / values as a wave holds them: what was loaded, and the operand of one product from it.  Addresses are a uniform base (scalar
+// registers) plus one 32-bit offset per lane that never changes.
+template <typename V> __device__ __forceinline__ V ld_at(const void* base, unsigned off) { return *reinterpret_cast<const V*>((const char*)base + off); }
+
 template <int KIND, int D> struct KeyTile {       // bf16, f32: octets of the U x 2 rows this lane stands for
-    static constexpr int U = KvT<KIND>::TK / 32;
+    static constexpr int U = tile_u(KIND, D), EB = KIND == KV_F32 ? 4 : 2;
     typename KvT<KIND>::frag_t f[U][2][D / 32];
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
-        typedef typename KvT<KIND>::row_t T;
-        const T* base = (const T*)p.kc + ((head << p.r.ps_log2) + at + (l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8;
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return (((l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8) * EB; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+        const char* base = (const char*)p.kc + ((head << p.r.ps_log2) + at) * D * EB;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int s = 0; s < D / 32; ++s) f[u][t][s] = *reinterpret_cast<const typename KvT<KIND>::frag_t*>(base + (u * 8 + t * 4) * D + s * 32);
+                for (int s = 0; s < D / 32; ++s) f[u][t][s] = ld_at<typename KvT<KIND>::frag_t>(base + ((u * 8 + t * 4) * D + s * 32) * EB, off);
     }
     __device__ __forceinline__ typename KvT<KIND>::frag_t get(int u, int t, int s) const { return f[u][t][s]; }
 };
 template <int KIND, int D> struct ValTile {
-    static constexpr int U = KvT<KIND>::TK / 32;
+    static constexpr int U = tile_u(KIND, D), EB = KIND == KV_F32 ? 4 : 2;
     typename KvT<KIND>::frag_t f[D / 16][U];
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
-        typedef typename KvT<KIND>::row_t T;
-        const T* base = (const T*)p.vc + ((head * D + l15) << p.r.ps_log2) + at + g * 8 * U;
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g, int ps_log2) { return ((l15 << ps_log2) + g * 8 * U) * EB; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+        const char* base = (const char*)p.vc + (((head * D) << p.r.ps_log2) + at) * EB;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-            for (int u = 0; u < U; ++u) f[d][u] = *reinterpret_cast<const typename KvT<KIND>::frag_t*>(base + ((long)d * 16 << p.r.ps_log2) + u * 8);
+            for (int u = 0; u < U; ++u) f[d][u] = ld_at<typename KvT<KIND>::frag_t>(base + ((d * 16 << p.r.ps_log2) + u * 8) * EB, off);
+    }
+    __device__ __forceinline__ void mask(int pos, int lo, int hi) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const OctetBits<typename KvT<KIND>::frag_t> bits(pos + u * 8, lo, hi);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) f[d][u] = bits.keep(f[d][u]);
+        }
     }
     __device__ __forceinline__ typename KvT<KIND>::frag_t get(int d, int u) const { return f[d][u]; }
 };
 template <int D> struct KeyTile<KV_INT4, D> {
-    static constexpr int U = 2, NS = D / 32;
-    unsigned w[U][2][NS], m[U][2][NS];
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
-        const long row = (head << p.r.ps_log2) + at + (l15 >> 2) * 8 * U + (l15 & 3);
-        const unsigned* base = (const unsigned*)p.kc + row * (D / 8) + g * NS;
-        const unsigned* meta = (const unsigned*)p.km + row * NS;
+    static constexpr int U = tile_u(KV_INT4, D), NS = D / 32;
+    typedef unsigned words_t __attribute__((ext_vector_type(NS)));
+    words_t w[U][2], m[U][2];
+    // codes at `off`, scales and zeros at off / D * 8: rows are D / 2 and D / 8 bytes
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return ((l15 >> 2) * 8 * U + (l15 & 3)) * (D / 2) + g * NS * 4; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+        const long row = (head << p.r.ps_log2) + at;
+        const char* base = (const char*)p.kc + row * (D / 2);
+        const char* meta = (const char*)p.km + row * (D / 8);
+        const unsigned moff = off / (D / 2) * (D / 8);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                __builtin_memcpy(w[u][t], __builtin_assume_aligned(base + (u * 8 + t * 4) * (D / 8), NS * 4 > 16 ? 16 : NS * 4), NS * 4);
-                __builtin_memcpy(m[u][t], __builtin_assume_aligned(meta + (u * 8 + t * 4) * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
+                w[u][t] = ld_at<words_t>(base + (u * 8 + t * 4) * (D / 2), off);
+                m[u][t] = ld_at<words_t>(meta + (u * 8 + t * 4) * (D / 8), moff);
             }
     }
     __device__ __forceinline__ f16x8_t get(int u, int t, int s) const { return dequant_key(w[u][t][s], m[u][t][s]); }
 };
 template <int D> struct ValTile<KV_INT4, D> {
-    static constexpr int U = 2;
-    unsigned w[D / 16][U];
+    static constexpr int U = tile_u(KV_INT4, D);
+    typedef unsigned words_t __attribute__((ext_vector_type(U)));
+    words_t w[D / 16];
     f16x8_t s[D / 32][U], z[D / 32][U];
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, int l15, int g) {
-        const unsigned* base = (const unsigned*)p.vc + ((head * D + l15) << (p.r.ps_log2 - 3)) + (at >> 3) + g * U;
-        const _Float16* meta = p.vm + ((head * (D / 32) * 2) << p.r.ps_log2) + at + g * 8 * U;
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g, int ps_log2) { return (l15 << (ps_log2 - 1)) + g * U * 4; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+        const char* base = (const char*)p.vc + ((head * D) << (p.r.ps_log2 - 1)) + (at >> 1);
+        const _Float16* meta = p.vm + ((head * (D / 32) * 2) << p.r.ps_log2) + at;
+        const unsigned moff = (off & 31) * 4;      // g * 8 U positions of 2 bytes (a channel's row is a multiple of 32 bytes)
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) __builtin_memcpy(w[d], __builtin_assume_aligned(base + ((long)d * 16 << (p.r.ps_log2 - 3)), U * 4), U * 4);
+        for (int d = 0; d < D / 16; ++d) w[d] = ld_at<words_t>(base + (d * 16 << (p.r.ps_log2 - 1)), off);
 #pragma unroll
         for (int k = 0; k < D / 32; ++k)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                s[k][u] = *reinterpret_cast<const f16x8_t*>(meta + ((long)(2 * k) << p.r.ps_log2) + u * 8);
-                z[k][u] = *reinterpret_cast<const f16x8_t*>(meta + ((long)(2 * k + 1) << p.r.ps_log2) + u * 8);
+                s[k][u] = ld_at<f16x8_t>(meta + ((2 * k) << p.r.ps_log2) + u * 8, moff);
+                z[k][u] = ld_at<f16x8_t>(meta + ((2 * k + 1) << p.r.ps_log2) + u * 8, moff);
             }
+    }
+    __device__ __forceinline__ void mask(int pos, int lo, int hi) {     // scale and zero 0: a value of 0 whatever the code
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const OctetBits<f16x8_t> bits(pos + u * 8, lo, hi);
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+                s[k][u] = bits.keep(s[k][u]);
+                z[k][u] = bits.keep(z[k][u]);
+            }
+        }
     }
     __device__ __forceinline__ f16x8_t get(int d, int u) const { return dequant_val(w[d][u], s[d >> 1][u], z[d >> 1][u]); }
 };
@@ -260,6 +296,72 @@ __device__ __forceinline__ void probs(const float (&x)[8], bf16x8_t& hi) {
     for (int e = 0; e < 8; ++e) hi[e] = (__bf16)x[e];
 }
 
+// The running maximum is raised only when a score exceeds it by more than 8 (in log2): P stays below 2^8, sums and products are f32, so nothing is lost,
+// and the usual step needs no cross-lane maximum and no rescaling.
+constexpr float MAX_SLACK = 8.f;
+constexpr float NO_MAX = -3e38f;                  // finite, so that masked scores (-inf) minus it stay -inf
+
+__device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// scores of a tile -> softmax step and products with the tile's values
+template <int KIND, int D>
+__device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2], const ValTile<KIND, D>& vt, float sc, float& m, float& l, f32x4_t (&acc)[D / 16]) {
+    typedef typename KvT<KIND>::frag_t frag_t;
+    constexpr int U = tile_u(KIND, D), ND = D / 16;
+    float x[U][8], mx = NO_MAX;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[u][e] = fmaf(s[u][e >> 2][e & 3], sc, -m);
+            mx = fmaxf(mx, x[u][e]);
+        }
+    if (__any(mx > MAX_SLACK)) {
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[u][e >> 2][e & 3] * sc);
+        mn = max_over_groups(mn);
+        const float a = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= a;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[u][e] = fmaf(s[u][e >> 2][e & 3], sc, -mn);
+    }
+    frag_t ph[U];
+    bf16x8_t pl[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[u][e] = __builtin_amdgcn_exp2f(x[u][e]);
+            l += x[u][e];
+        }
+        probs(x[u], ph[u]);
+        if constexpr (KIND == KV_BF16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[u][e] -= (float)ph[u][e];
+            probs(x[u], pl[u]);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const frag_t v = vt.get(d, u);
+            acc[d] = mma(v, ph[u], acc[d]);
+            if constexpr (KIND == KV_BF16) acc[d] = mma(v, pl[u], acc[d]);
+        }
+    }
+}
+
 // ---- few rows per session: every wave streams its own tiles from memory into registers -----------------------------------------------------
 // grid (q_tiles * n_splits, Hkv, B), 4 waves; wave w takes the split's tiles w, w + 4, ...; the four partial softmaxes meet in LDS at the end.  Bound
 // by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
@@ -268,7 +370,7 @@ template <int KIND, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND>::frag_t frag_t;
-    constexpr int TK = KvT<KIND>::TK, U = TK / 32, NS = D / 32, ND = D / 16;
+    constexpr int U = tile_u(KIND, D), TK = 32 * U, NS = D / 32, ND = D / 16;
     __shared__ float so[2][16][D + 4];
     __shared__ float sm[4][16], sl[4][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
@@ -289,18 +391,19 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
     f32x4_t acc[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    float m = NO_MAX, l = 0.f;
 
     int kb = k0 + wave * TK;
     if (kb < k1) {
         KeyTile<KIND, D> kt;
         ValTile<KIND, D> vt;
         const int ps_mask = (1 << p.r.ps_log2) - 1;
+        const unsigned k_off = KeyTile<KIND, D>::lane_off(l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
         int page = page_raw(p.r, b, kb), next = kb + 4 * TK < k1 ? page_raw(p.r, b, kb + 4 * TK) : -1;
         {
             const long head = (long)(page_ok(p.r, page) ? page : 0) * p.r.Hkv + hk;
-            kt.load(p, head, kb & ps_mask, l15, g);
-            vt.load(p, head, kb & ps_mask, l15, g);
+            kt.load(p, head, kb & ps_mask, k_off);
+            vt.load(p, head, kb & ps_mask, v_off);
         }
         for (; kb < k1; kb += 4 * TK) {
             const int nb = kb + 4 * TK;
@@ -316,57 +419,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
 #pragma unroll
                     for (int k = 0; k < NS; ++k) s[u][tt] = mma(kt.get(u, tt, k), q[k], s[u][tt]);
                 }
-            if (nb < k1) kt.load(p, nhead, nat, l15, g);
+            if (nb < k1) kt.load(p, nhead, nat, k_off);
             if (page_ok(p.r, page)) {
-                const bool edge = kb < sp.lo_all || kb + TK > sp.hi_all;
-                const int pos = kb + g * 8 * U;
-                float x[U][8], mx = -INFINITY;
+                if (kb < sp.lo_all || kb + TK > sp.hi_all) {
+                    const int pos = kb + g * 8 * U;
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                    for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[u][e] = s[u][e >> 2][e & 3] * sc;
-                        if (edge && (pos + u * 8 + e < c_lo || pos + u * 8 + e >= c_hi)) x[u][e] = -INFINITY;
-                        mx = fmaxf(mx, x[u][e]);
-                    }
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m, mx);
-                const float ms = mn == -INFINITY ? 0.f : mn;
-                if (__any(mn > m)) {
-                    const float a = __builtin_amdgcn_exp2f(m - ms);
-                    l *= a;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) acc[d] *= a;
+                        for (int e = 0; e < 8; ++e)
+                            if (pos + u * 8 + e < c_lo || pos + u * 8 + e >= c_hi) s[u][e >> 2][e & 3] = -INFINITY;
+                    vt.mask(pos, sp.lo, sp.hi);
                 }
-                m = mn;
-                frag_t ph[U];
-                bf16x8_t pl[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[u][e] = __builtin_amdgcn_exp2f(x[u][e] - ms);
-                        l += x[u][e];
-                    }
-                    probs(x[u], ph[u]);
-                    if constexpr (KIND == KV_BF16) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[u][e] -= (float)ph[u][e];
-                        probs(x[u], pl[u]);
-                    }
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        frag_t v = vt.get(d, u);
-                        if (edge) keep_range(v, pos + u * 8, sp.lo, sp.hi);
-                        acc[d] = mma(v, ph[u], acc[d]);
-                        if constexpr (KIND == KV_BF16) acc[d] = mma(v, pl[u], acc[d]);
-                    }
+                step_tile<KIND, D>(s, vt, sc, m, l, acc);
             }
-            if (nb < k1) vt.load(p, nhead, nat, l15, g);
+            if (nb < k1) vt.load(p, nhead, nat, v_off);
             page = next;
             next = after;
         }
@@ -381,11 +447,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
     }
     __syncthreads();
     float M = fmaxf(fmaxf(sm[0][l15], sm[1][l15]), fmaxf(sm[2][l15], sm[3][l15]));
-    const float Ms = M == -INFINITY ? 0.f : M;
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L += sl[w][l15] * __builtin_amdgcn_exp2f(sm[w][l15] - Ms);
-    const float mine = __builtin_amdgcn_exp2f(m - Ms);
+    for (int w = 0; w < 4; ++w) L += sl[w][l15] * __builtin_amdgcn_exp2f(sm[w][l15] - M);
+    const float mine = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] *= mine;
 #pragma unroll
@@ -422,85 +487,173 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
 // float16), a double buffer and one barrier per tile.  Octets are stored at index o ^ f(row): the 8 lanes that read together hold rows whose f differs,
 // so the 16-byte reads hit every bank once.  Per 32 positions a wave reads 2 KiB x D / 64 of keys and of values for 16 NC columns; at NC = 2 the LDS reads
 // take as long as the products.
-//
-// The running maximum is raised only when a score exceeds it by more than 8 (in log2): P stays below 2^8, sums and products are f32, so nothing is lost,
-// and the usual step needs no cross-lane maximum and no rescaling.
-constexpr float MAX_SLACK = 8.f;
-constexpr float NO_MAX = -3e38f;                  // finite, so that masked scores (-inf) minus it stay -inf
-
-__device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 template <int KIND, int D> struct LdsTile {
-    typedef typename KvT<KIND>::frag_t frag_t;
-    static constexpr int TK = KvT<KIND>::TK, U = TK / 32;
-    static constexpr int EB = KIND == KV_F32 ? 4 : 2;              // bytes per element in LDS
+    static constexpr int U = tile_u(KIND, D), TK = 32 * U;
+    static constexpr int EB = KIND == KV_F32 ? 4 : 2, OB = 8 * EB;  // bytes per element and per octet in LDS
     static constexpr int K_BYTES = TK * D * EB, BYTES = 2 * K_BYTES;
-    static __device__ __forceinline__ int kf(int key) { return (key & 3) | ((key >> (U == 2 ? 4 : 3)) & 1) << 2; }
+    static constexpr int FB = U == 2 ? 4 : 3;                      // position bit that is bit 2 of its f
+    static __device__ __forceinline__ int kf(int key) { return (key & 3) | ((key >> FB) & 1) << 2; }
     static __device__ __forceinline__ int vf(int d) { return d & (TK / 8 - 1); }
-    static __device__ __forceinline__ int k_at(int key, int o) { return (key * (D / 8) + (o ^ kf(key))) * 8 * EB; }
-    static __device__ __forceinline__ int v_at(int d, int o) { return K_BYTES + (d * (TK / 8) + (o ^ vf(d))) * 8 * EB; }
+    static __device__ __forceinline__ int k_at(int key, int o) { return (key * (D / 8) + (o ^ kf(key))) * OB; }
+    static __device__ __forceinline__ int v_at(int d, int o) { return K_BYTES + (d * (TK / 8) + (o ^ vf(d))) * OB; }
+};
+// The reading side: f of a lane's key rows is l15 % 8 and of its value rows l15 % (TK / 8), whatever the product, so four lane offsets serve all reads
+// and the rest are constants: octet 4 k + g of a key row lies 4 OB (k ^ f / 4) behind octet (g ^ f % 4).
+template <int KIND, int D> struct LdsOff {
+    typedef LdsTile<KIND, D> L;
+    int k[2], v[L::U];
+    __device__ __forceinline__ LdsOff(int l15, int g) {
+        const int key = (l15 >> 2) * 8 * L::U + (l15 & 3);
+        k[0] = L::k_at(key, g);                    // even k: + 4 OB k
+        k[1] = L::k_at(key, 4 + g) - 4 * L::OB;    // odd k: + 4 OB k
+#pragma unroll
+        for (int u = 0; u < L::U; ++u) v[u] = L::v_at(l15, g * L::U + u);
+    }
 };
 
-// page -> LDS: 16-byte pieces in LDS order, the swizzle in the source address
-template <int KIND, int D>
-__device__ __forceinline__ void tile_dma(const PagedAttn& p, unsigned char* buf, int page, int hk, int at, int wave, int lane) {
+// page -> LDS: 16-byte pieces in LDS order, the swizzle in the lane's source offset (which changes with the piece only by f's bit 2)
+template <int KIND, int D> struct TileDma {
     typedef LdsTile<KIND, D> L;
-    constexpr int PB = L::EB / 2;                                  // pieces per octet
-    constexpr int N = L::K_BYTES / 16 / 256;                       // pieces per thread, keys or values
-    const long head = (long)page * p.r.Hkv + hk;
-    const unsigned char* kb = (const unsigned char*)p.kc + ((head << p.r.ps_log2) + at) * D * L::EB;
-    const unsigned char* vb = (const unsigned char*)p.vc + (((head * D) << p.r.ps_log2) + at) * L::EB;
+    static constexpr int PB = L::EB / 2;                           // pieces per octet
+    static constexpr int N = L::K_BYTES / 16 / 256;                // pieces per thread, keys or values
+    static constexpr int KS = 256 / PB / (D / 8);                  // key rows per piece of the workgroup
+    static constexpr int VS = 256 / PB / (L::TK / 8);              // value rows
+    unsigned k[2], v;
+    __device__ __forceinline__ TileDma(int tid, int ps_log2) {
+        const int o = tid / PB, half = tid % PB;
+        const int key = o / (D / 8), d = o / (L::TK / 8);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c0 = (i * 4 + wave) * 64, c = c0 + lane, o = c / PB, half = c % PB;
-        const int key = o / (D / 8), ko = (o % (D / 8)) ^ L::kf(key);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + (long)(key * D + ko * 8) * L::EB + half * 16),
-                                         (__attribute__((address_space(3))) void*)(buf + c0 * 16), 16, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c0 = (i * 4 + wave) * 64, c = c0 + lane, o = c / PB, half = c % PB;
-        const int d = o / (L::TK / 8), vo = (o % (L::TK / 8)) ^ L::vf(d);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + (((long)d << p.r.ps_log2) + vo * 8) * L::EB + half * 16),
-                                         (__attribute__((address_space(3))) void*)(buf + L::K_BYTES + c0 * 16), 16, 0, 0);
-    }
-}
-// 4-bit page -> registers: D / 32 octets of one key and D / 32 octets of one value channel per thread, with their scales and zeros
-template <int D> struct CodeRegs {
-    static constexpr int NS = D / 32;
-    unsigned kw[NS], km[NS], vw[NS];
-    f16x8_t vs[NS], vz[NS];
-    __device__ __forceinline__ void load(const PagedAttn& p, int page, int hk, int at, int tid) {
-        const long head = (long)page * p.r.Hkv + hk;
-        const int key = tid >> 2, g = tid & 3, d = tid * NS / 8, o = tid * NS % 8;
-        const long row = (head << p.r.ps_log2) + at + key;
-        __builtin_memcpy(kw, __builtin_assume_aligned((const unsigned*)p.kc + row * (D / 8) + g * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
-        __builtin_memcpy(km, __builtin_assume_aligned((const unsigned*)p.km + row * NS, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
-        __builtin_memcpy(vw, __builtin_assume_aligned((const unsigned*)p.vc + ((head * D + d) << (p.r.ps_log2 - 3)) + (at >> 3) + o, NS * 4 > 16 ? 16 : NS * 4), NS * 4);
-        const _Float16* m = p.vm + ((head * NS + d / 32) * 2 << p.r.ps_log2) + at + o * 8;
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            vs[j] = *reinterpret_cast<const f16x8_t*>(m + j * 8);
-            vz[j] = *reinterpret_cast<const f16x8_t*>(m + ((long)1 << p.r.ps_log2) + j * 8);
+        for (int bit = 0; bit < 2; ++bit) {
+            const int f = (key & 3) | (KS > (1 << L::FB) ? (key >> L::FB) & 1 : bit) << 2;
+            k[bit] = (key * D + ((o % (D / 8)) ^ f) * 8) * L::EB + half * 16;
         }
+        v = (((unsigned)d << ps_log2) + ((o % (L::TK / 8)) ^ L::vf(d)) * 8) * L::EB + half * 16;
+    }
+    __device__ __forceinline__ void start(const PagedAttn& p, unsigned char* buf, int page, int hk, int at, int wave) const {
+        const long head = (long)page * p.r.Hkv + hk;
+        const char* kb = (const char*)p.kc + ((head << p.r.ps_log2) + at) * D * L::EB;
+        const char* vb = (const char*)p.vc + (((head * D) << p.r.ps_log2) + at) * L::EB;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + i * KS * D * L::EB + k[((i * KS) >> L::FB) & 1]),
+                                             (__attribute__((address_space(3))) void*)(buf + (i * 4 + wave) * 1024), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + (((long)i * VS) << p.r.ps_log2) * L::EB + v),
+                                             (__attribute__((address_space(3))) void*)(buf + L::K_BYTES + (i * 4 + wave) * 1024), 16, 0, 0);
+    }
+};
+// 4-bit page -> registers: TK D / 2048 octets of one key; and as many octets of the same 8 positions, channels of one group, which share 8 scales and zeros
+template <int D> struct CodeRegs {
+    typedef LdsTile<KV_INT4, D> L;
+    static constexpr int NS = D / 32, KN = L::TK * D / 2048, KT = NS * 4 / KN;     // octets per thread; threads per key
+    static constexpr int VT = L::TK / 8;                                           // threads per channel
+    typedef unsigned words_t __attribute__((ext_vector_type(KN)));
+    words_t kw;
+    unsigned km[KN], vw[KN];
+    f16x8_t vs, vz;
+    // dword i of a key row is octet 4 s + g with g = i / NS, s = i % NS
+    __device__ __forceinline__ void load(const PagedAttn& p, int page, int hk, int at, int tid) {
+        const long head = (long)page * p.r.Hkv + hk, row = (head << p.r.ps_log2) + at;
+        const int key = tid / KT, i0 = tid % KT * KN, o = tid % VT, d0 = tid / VT * KN;
+        kw = ld_at<words_t>((const char*)p.kc + row * (D / 2), key * (D / 2) + i0 * 4);
+#pragma unroll
+        for (int j = 0; j < KN; ++j) km[j] = ld_at<unsigned>((const char*)p.km + row * (D / 8), key * (D / 8) + (i0 + j) % NS * 4);
+        const char* vb = (const char*)p.vc + ((head * D) << (p.r.ps_log2 - 1)) + (at >> 1);
+#pragma unroll
+        for (int j = 0; j < KN; ++j) vw[j] = ld_at<unsigned>(vb, ((d0 + j) << (p.r.ps_log2 - 1)) + o * 4);
+        const char* m = (const char*)(p.vm + ((head * NS * 2) << p.r.ps_log2) + at);
+        const unsigned moff = ((d0 / 32 * 2) << p.r.ps_log2) * 2 + o * 16;
+        vs = ld_at<f16x8_t>(m, moff);
+        vz = ld_at<f16x8_t>(m, moff + (2u << p.r.ps_log2));
     }
     __device__ __forceinline__ void store(unsigned char* buf, int tid) const {
-        typedef LdsTile<KV_INT4, D> L;
-        const int key = tid >> 2, g = tid & 3, d = tid * NS / 8, o = tid * NS % 8;
+        const int key = tid / KT, i0 = tid % KT * KN, o = tid % VT, d0 = tid / VT * KN;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) *reinterpret_cast<f16x8_t*>(buf + L::k_at(key, 4 * s + g)) = dequant_key(kw[s], km[s]);
+        for (int j = 0; j < KN; ++j) *reinterpret_cast<f16x8_t*>(buf + L::k_at(key, 4 * ((i0 + j) % NS) + (i0 + j) / NS)) = dequant_key(kw[j], km[j]);
 #pragma unroll
-        for (int j = 0; j < NS; ++j) *reinterpret_cast<f16x8_t*>(buf + L::v_at(d, o + j)) = dequant_val(vw[j], vs[j], vz[j]);
+        for (int j = 0; j < KN; ++j) *reinterpret_cast<f16x8_t*>(buf + L::v_at(d0 + j, o)) = dequant_val(vw[j], vs, vz);
     }
 };
 
+// one tile: scores, softmax step, products with the values, 32 positions at a time
 template <int KIND, int D, int NC>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(PagedAttn p) {
+__device__ __forceinline__ void tile_step(const unsigned char* buf, const LdsOff<KIND, D>& off, const typename KvT<KIND>::frag_t (&q)[NC][D / 32], const float (&sc)[NC],
+                                          bool edge, int pos0, const int (&c_lo)[NC], const int (&c_hi)[NC], float (&m)[NC], float (&l)[NC], f32x4_t (&acc)[NC][D / 16]) {
+    typedef typename KvT<KIND>::frag_t frag_t;
+    typedef LdsTile<KIND, D> L;
+    constexpr int U = L::U, NS = D / 32, ND = D / 16;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pos = pos0 + u * 8;
+        f32x4_t s[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+            for (int k = 0; k < NS; ++k) {
+                const frag_t a = *reinterpret_cast<const frag_t*>(buf + off.k[k & 1] + ((u * 8 + tt * 4) * (D / 8) + 4 * k) * L::OB);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[c][tt] = mma(a, q[c][k], s[c][tt]);
+            }
+        }
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (pos + e < c_lo[c] || pos + e >= c_hi[c]) s[c][e >> 2][e & 3] = -INFINITY;
+        }
+        float x[NC][8];
+        bool raise = false;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float mx = NO_MAX;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -m[c]);
+                mx = fmaxf(mx, x[c][e]);
+            }
+            raise |= mx > MAX_SLACK;
+        }
+        if (__any(raise)) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                float mn = m[c];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[c][e >> 2][e & 3] * sc[c]);
+                mn = max_over_groups(mn);
+                const float a = __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= a;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) acc[c][d] *= a;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -mn);
+            }
+        }
+        frag_t pr[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
+                l[c] += x[c][e];
+            }
+            probs(x[c], pr[c]);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            const frag_t v = *reinterpret_cast<const frag_t*>(buf + off.v[u] + d * 16 * (L::TK / 8) * L::OB);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) acc[c][d] = mma(v, pr[c], acc[c][d]);
+        }
+    }
+}
+
+template <int KIND, int D, int NC>
+__global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_paged_tile_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND>::frag_t frag_t;
     typedef LdsTile<KIND, D> L;
@@ -528,12 +681,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(
 
     frag_t q[NC][NS];
     float sc[NC], m[NC], l[NC];
+    int c_lo[NC], c_hi[NC];
     f32x4_t acc[NC][ND];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int vr = vr0 + wave * RW + c * 16 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
         load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, vr < nvr, p.q_vec, g, q[c], sc[c]);
         sc[c] *= p.scale_log2e;
+        c_hi[c] = p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
+        c_lo[c] = p.window > 0 ? sp.past + t + 1 - p.window : 0;
         m[c] = NO_MAX;
         l[c] = 0.f;
 #pragma unroll
@@ -543,7 +699,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(
     const int ps_mask = (1 << p.r.ps_log2) - 1;
     int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, cur = 0;
     int next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1;
-    CodeRegs<KIND == KV_INT4 ? D : 32> regs;
+    CodeRegs<D> regs;
+    const LdsOff<KIND, D> off(l15, g);
+    const TileDma<KIND == KV_INT4 ? KV_BF16 : KIND, D> dma(tid, p.r.ps_log2);
     if constexpr (KIND == KV_INT4) {
         if (page_ok(p.r, page)) {
             regs.load(p, page, hk, k0 & ps_mask, tid);
@@ -551,7 +709,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(
         }
         if (page_ok(p.r, next)) regs.load(p, next, hk, (k0 + TK) & ps_mask, tid);
     } else {
-        if (page_ok(p.r, page)) tile_dma<KIND, D>(p, lds, page, hk, k0 & ps_mask, wave, lane);
+        if (page_ok(p.r, page)) dma.start(p, lds, page, hk, k0 & ps_mask, wave);
     }
     for (int kb = k0; kb < k1; kb += TK) {
         __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed
@@ -563,79 +721,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_tile_kernel(
             if (page_ok(p.r, next)) regs.store(other, tid);
             if (page_ok(p.r, after)) regs.load(p, after, hk, (kb + 2 * TK) & ps_mask, tid);
         } else {
-            if (page_ok(p.r, next)) tile_dma<KIND, D>(p, other, next, hk, (kb + TK) & ps_mask, wave, lane);
+            if (page_ok(p.r, next)) dma.start(p, other, next, hk, (kb + TK) & ps_mask, wave);
+        }
+        if (kb < sp.lo || kb + TK > sp.hi) {       // the first and last tile: values nobody attends to become 0 where they lie
+            for (int i = tid; i < D * TK / 8; i += 256) {
+                const int d = i / (TK / 8), o = i % (TK / 8);
+                frag_t* v = reinterpret_cast<frag_t*>(lds + cur * L::BYTES + L::v_at(d, o));
+                *v = OctetBits<frag_t>(kb + o * 8, sp.lo, sp.hi).keep(*v);
+            }
+            __syncthreads();
         }
         if (page_ok(p.r, page) && kb < sw.hi && kb + TK > sw.lo) {
-            const bool edge = kb < sw.lo_all || kb + TK > sw.hi_all;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                f32x4_t s[NC][2];
-#pragma unroll
-                for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const int key = (l15 >> 2) * 8 * U + u * 8 + tt * 4 + (l15 & 3);
-#pragma unroll
-                    for (int k = 0; k < NS; ++k) {
-                        const frag_t a = *reinterpret_cast<const frag_t*>(buf + L::k_at(key, 4 * k + g));
-#pragma unroll
-                        for (int c = 0; c < NC; ++c) s[c][tt] = mma(a, q[c][k], s[c][tt]);
-                    }
-                }
-                const int pos = kb + g * 8 * U + u * 8;
-                float x[NC][8];
-                bool raise = false;
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    if (edge) {
-                        const int t = (vr0 + wave * RW + c * 16 + l15) / p.G;
-                        const int hi = p.causal ? min(sp.len, sp.past + t + 1) : sp.len, lo = p.window > 0 ? sp.past + t + 1 - p.window : 0;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (pos + e < lo || pos + e >= hi) s[c][e >> 2][e & 3] = -INFINITY;
-                    }
-                    float mx = NO_MAX;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -m[c]);
-                        mx = fmaxf(mx, x[c][e]);
-                    }
-                    raise |= mx > MAX_SLACK;
-                }
-                if (__any(raise)) {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        float mx = m[c];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[c][e >> 2][e & 3] * sc[c]);
-                        mx = max_over_groups(mx);
-                        const float a = __builtin_amdgcn_exp2f(m[c] - mx);
-                        m[c] = mx;
-                        l[c] *= a;
-#pragma unroll
-                        for (int d = 0; d < ND; ++d) acc[c][d] *= a;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -mx);
-                    }
-                }
-                frag_t pr[NC];
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
-                        l[c] += x[c][e];
-                    }
-                    probs(x[c], pr[c]);
-                }
-#pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    frag_t v = *reinterpret_cast<const frag_t*>(buf + L::v_at(d * 16 + l15, g * U + u));
-                    if (edge) keep_range(v, pos, sp.lo, sp.hi);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) acc[c][d] = mma(v, pr[c], acc[c][d]);
-                }
-            }
+            tile_step<KIND, D, NC>(buf, off, q, sc, kb < sw.lo_all || kb + TK > sw.hi_all, kb + g * 8 * U, c_lo, c_hi, m, l, acc);
         }
         page = next;
         next = after;
@@ -702,15 +799,15 @@ struct PagedPlan {
     int n_splits, chunk, q_tiles;
     bool tile;                    // attn_paged_tile_kernel
 };
-constexpr int tile_nc(int kind, int D) { return D == 256 && kind != KV_BF16 ? 1 : 2; }     // 256 channels: what the registers hold
+constexpr int tile_nc(int D) { return D == 256 ? 1 : 2; }           // 256 channels: what the registers hold
 // Which kernel, how many query tiles and splits: enough workgroups for two on every CU, no split shorter than 256 positions (a tile per wave).
 static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, int max_kv, int causal, int window) {
     PagedPlan pl;
     const int G = H / kv->kv_heads;
     pl.tile = (long)max_new * G > 32;
-    const int rows = pl.tile ? 4 * 16 * tile_nc(paged_kind(kv), kv->head_dim) : 16;
+    const int rows = pl.tile ? 4 * 16 * tile_nc(kv->head_dim) : 16;
     pl.q_tiles = cdiv((long)max_new * G, rows);
-    const long span = std::min<long>(max_kv, causal && window > 0 ? (long)window + cdiv(rows - 1, G) + 1 + 63 : max_kv) + 63;
+    const long span = causal && window > 0 ? std::min<long>(max_kv, (long)window + cdiv(rows - 1, G) + 1 + 63) + 63 : max_kv;      // from a multiple of 64
     const long groups = (long)B * kv->kv_heads * pl.q_tiles;
     const long want = std::max<long>(1, 1024 / std::max<long>(1, groups));
     pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
@@ -720,7 +817,7 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
 }
 
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
-    if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(KIND, D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
+    if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
     else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
     if (p.n_splits > 1) attn_paged_join_kernel<T, D><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }

@@ -36,16 +36,22 @@ def _require(cond, msg: str) -> None:
         raise ValueError(msg)
 
 
+# The checks of a call's tensors cost as much as its launch: they are plain comparisons, and a message is put together only to be raised.
+
+
 class _on_device:
-    """Make the tensors' device current for the call (a no-op where it is: the usual case, and cheaper than torch's guard)."""
+    """Make the tensors' device current for the call (nothing where it is) and give torch's current stream there."""
 
     def __init__(self, device):
-        _require(device.type == "cuda", f"tensors on {device}: the operators run on a GPU only")
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"tensors on {device}: the operators run on a GPU only")
+        self.index = device.index
+        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard:
             self.guard.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.guard:
@@ -53,15 +59,19 @@ class _on_device:
 
 
 def _ints(t, n, device, what):
-    _require(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous() and t.device == device,
-             f"{what}: contiguous int32[{n}] on {device} needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what}: contiguous int32[{n}] on {device} needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _rows(t, heads, dim, dtype, device, what):
-    """[rows][heads][dim] whose heads lie next to each other (a slice of a fused projection's rows is fine)."""
-    _require(t.dim() == 3 and t.shape[2] == dim and t.dtype == dtype and t.device == device and (heads is None or t.shape[1] == heads),
-             f"{what}: {dtype} [rows][{'heads' if heads is None else heads}][{dim}] on {device} needed, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    _require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == dim)), f"{what}: the heads of a row must lie next to each other")
+    """[rows][heads][dim] whose heads lie next to each other (a slice of a fused projection's rows is fine) -> (rows, heads, row stride)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or t.dtype is not dtype or t.device != device or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: {dtype} [rows][{'heads' if heads is None else heads}][{dim}] on {device} needed, got {t.dtype} {tuple(shape)} on {t.device}")
+    rs, hs, ds = t.stride()
+    if (ds != 1 or (hs != dim and shape[1] != 1)) and t.numel():
+        raise ValueError(f"{what}: the heads of a row must lie next to each other, got strides {(rs, hs, ds)}")
+    return shape[0], shape[1], rs
 
 
 def rope_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, original: int = 0):
@@ -100,25 +110,31 @@ def rope_tables(rotary_dim: int, max_pos: int, theta: float = 10000.0, *, scalin
     return (a.cos() * m).float().to(device), (a.sin() * m).float().to(device)
 
 
-def _check_tables(cos, sin, device):
-    _require(cos is not None and sin is not None and cos.dim() == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype == torch.float32
-             and cos.is_contiguous() and sin.is_contiguous() and cos.device == device and sin.device == device,
-             f"cos / sin: contiguous float32 [max_pos][rotary_dim / 2] on {device} needed")
+def _tables(cos, sin, device):
+    """-> (positions, channels that turn, cos pointer, sin pointer)."""
+    if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
+            or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != device or sin.device != device:
+        raise ValueError(f"cos / sin: contiguous float32 [max_pos][rotary_dim / 2] on {device} needed")
+    n, half = cos.shape
+    return n, 2 * half, cos.data_ptr(), sin.data_ptr()
 
 
 def rope(x, positions, cos, sin, *, interleaved: bool = False, out=None):
     """Turn the first ``2 * cos.shape[1]`` channels of every head of ``x`` [rows][heads][dim] to its row's position -> ``out`` (new, or given, or
     ``x`` itself).  ``positions`` int32 [rows]: a negative one leaves the row of ``out`` as it is, one behind the table gives NaN."""
-    _require(x.dim() == 3 and (x.numel() == 0 or x.stride(2) == 1), "x: [rows][heads][dim] with neighbouring channels needed")
-    _ints(positions, x.shape[0], x.device, "positions")
-    _check_tables(cos, sin, x.device)
+    device, shape = x.device, x.shape
+    if len(shape) != 3 or (x.stride(2) != 1 and x.numel()):
+        raise ValueError(f"x: [rows][heads][dim] with neighbouring channels needed, got {tuple(shape)}, strides {x.stride()}")
+    _ints(positions, shape[0], device, "positions")
+    n, rot, cp, sp = _tables(cos, sin, device)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _require(out.shape == x.shape and out.dtype == x.dtype and out.device == x.device and (x.numel() == 0 or out.stride(2) == 1), "out must match x")
-    with _on_device(x.device):
-        native.check(native.load().s2s_op_rope(native.stream_handle(), x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                                               positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0], x.shape[0], x.shape[1], x.shape[2],
-                                               2 * cos.shape[1], 1 if interleaved else 0, native.dtype_code(x.dtype)), "s2s_op_rope")
+        out = torch.empty(shape, dtype=x.dtype, device=device)
+    elif out.shape != shape or out.dtype is not x.dtype or out.device != device or (out.stride(2) != 1 and out.numel()):
+        raise ValueError(f"out must match x, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    xs, os = x.stride(), out.stride()
+    with _on_device(device) as stream:
+        native.check(native.load().s2s_op_rope(stream, x.data_ptr(), xs[0], xs[1], out.data_ptr(), os[0], os[1], positions.data_ptr(), cp, sp, n, shape[0], shape[1], shape[2], rot,
+                                               1 if interleaved else 0, native.dtype_code(x.dtype)), "s2s_op_rope")
     return out
 
 
@@ -163,39 +179,43 @@ class PagedKVCache:
         self._ref = C.byref(self._kv)
 
     def _sessions(self, table, lens, cu, rows, max_new, what):
-        _require(table.dtype == torch.int32 and table.dim() == 2 and table.is_contiguous() and table.device == self.device, f"table: contiguous int32 [sessions][pages] on {self.device} needed")
-        b = table.shape[0]
+        """-> (sessions, pages per session, bound of the new rows)."""
+        if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.device != self.device:
+            raise ValueError(f"table: contiguous int32 [sessions][pages] on {self.device} needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
+        b, cols = table.shape
         _ints(lens, b, self.device, what)
         if cu is None:
-            _require(rows == b and max_new in (None, 1), f"without cu there is one row per session ({rows} rows, {b} sessions)")
-            return b, 1
+            if rows != b or max_new not in (None, 1):
+                raise ValueError(f"without cu there is one row per session ({rows} rows, {b} sessions, max_new {max_new})")
+            return b, cols, 1
         _ints(cu, b + 1, self.device, "cu")
-        return b, max(1, rows if max_new is None else max_new)
+        return b, cols, max(1, rows if max_new is None else max_new)
 
     def append(self, k, v, table, start, cu=None, *, max_new=None, cos=None, sin=None, interleaved: bool = False, q=None, q_out=None):
         """Store every session's new rows behind the ``start`` positions its pages hold, keys turned to their positions (``cos`` / ``sin`` None: as they come).
         ``q`` is turned along -> ``q_out`` (new, or given, or ``q`` itself), which is returned."""
-        _rows(k, self.kv_heads, self.head_dim, self.dtype, self.device, "k")
-        _rows(v, self.kv_heads, self.head_dim, self.dtype, self.device, "v")
-        T = k.shape[0]
-        b, max_new = self._sessions(table, start, cu, T, max_new, "start")
-        _require(v.shape[0] == T and (q is None or q.shape[0] == T), "k, v and q need the same rows")
-        H = 0
-        if cos is not None or sin is not None:
-            _check_tables(cos, sin, self.device)
+        device, dim, dtype = self.device, self.head_dim, self.dtype
+        T, _, k_rs = _rows(k, self.kv_heads, dim, dtype, device, "k")
+        Tv, _, v_rs = _rows(v, self.kv_heads, dim, dtype, device, "v")
+        b, cols, max_new = self._sessions(table, start, cu, T, max_new, "start")
+        n, rot, cp, sp = (0, 0, 0, 0) if cos is None and sin is None else _tables(cos, sin, device)
+        Tq, H, q_rs, qp, qo_rs, qop = T, 0, 0, 0, 0, 0
         if q is not None:
-            _require(cos is not None, "queries are turned: cos / sin needed")
-            _rows(q, None, self.head_dim, self.dtype, self.device, "q")
-            H = q.shape[1]
+            if cos is None:
+                raise ValueError("queries are turned: cos / sin needed")
+            Tq, H, q_rs = _rows(q, None, dim, dtype, device, "q")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            _rows(q_out, H, self.head_dim, self.dtype, self.device, "q_out")
-            _require(q_out.shape[0] == T, "q_out needs q's rows")
-        with _on_device(self.device):
-            native.check(native.load().s2s_op_kv_append_paged(
-                native.stream_handle(), self._ref, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), native.ptr(q), q.stride(0) if H else 0, native.ptr(q_out) if H else 0,
-                q_out.stride(0) if H else 0, H, table.data_ptr(), table.shape[1], start.data_ptr(), native.ptr(cu), b, T, max_new, native.ptr(cos), native.ptr(sin),
-                cos.shape[0] if cos is not None else 0, 2 * cos.shape[1] if cos is not None else 0, 1 if interleaved else 0), "s2s_op_kv_append_paged")
+                q_out = torch.empty(q.shape, dtype=dtype, device=device)
+            To, _, qo_rs = _rows(q_out, H, dim, dtype, device, "q_out")
+            if To != Tq:
+                raise ValueError(f"q_out: {Tq} rows needed, got {To}")
+            qp, qop = q.data_ptr(), q_out.data_ptr()
+        if Tv != T or Tq != T:
+            raise ValueError(f"k, v and q need the same rows, got {T}, {Tv} and {Tq}")
+        with _on_device(device) as stream:
+            native.check(native.load().s2s_op_kv_append_paged(stream, self._ref, k.data_ptr(), k_rs, v.data_ptr(), v_rs, qp, q_rs, qop, qo_rs, H, table.data_ptr(), cols,
+                                                              start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, T, max_new, cp, sp, n, rot, 1 if interleaved else 0),
+                         "s2s_op_kv_append_paged")
         return q_out if H else None
 
     def read(self, table, start, cu=None, rows=None, *, max_new=None):
@@ -204,12 +224,13 @@ class PagedKVCache:
         if rows is None:
             _require(cu is None, "rows: how many rows cu counts")
             rows = table.shape[0]
-        b, max_new = self._sessions(table, start, cu, rows, max_new, "start")
-        out = torch.empty(2, rows, self.kv_heads, self.head_dim, dtype=self.dtype, device=self.device)
-        with _on_device(self.device):
-            native.check(native.load().s2s_op_kv_read_paged(native.stream_handle(), self._ref, table.data_ptr(), table.shape[1], start.data_ptr(), native.ptr(cu), b, rows, max_new,
-                                                            out[0].data_ptr(), out[1].data_ptr(), self.kv_heads * self.head_dim), "s2s_op_kv_read_paged")
-        return out[0], out[1]
+        b, cols, max_new = self._sessions(table, start, cu, rows, max_new, "start")
+        shape = (rows, self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
+        with _on_device(self.device) as stream:
+            native.check(native.load().s2s_op_kv_read_paged(stream, self._ref, table.data_ptr(), cols, start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, rows, max_new,
+                                                            k.data_ptr(), v.data_ptr(), self.kv_heads * self.head_dim), "s2s_op_kv_read_paged")
+        return k, v
 
     def workspace_bytes(self, heads: int, sessions: int, rows: int, *, max_new: int = 1, max_kv: int, causal: bool = True, window: int = 0) -> int:
         """Bytes ``attend`` needs beside its buffers for these sizes."""
@@ -223,23 +244,28 @@ class PagedKVCache:
         ``q`` [rows][heads][head_dim], heads a multiple of ``kv_heads``; ``scale`` None: head_dim ** -0.5.  causal: new row i of n sees the positions
         below kv_len - n + i + 1, ``window`` > 0: the last ``window`` of those.  A row that sees nothing is zero.  ``workspace``: uint8 tensor of
         ``workspace_bytes`` (None: taken from torch's allocator; one given to calls on several streams at once would be overwritten)."""
-        _rows(q, None, self.head_dim, self.dtype, self.device, "q")
-        T, H = q.shape[0], q.shape[1]
-        b, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
+        device, dim = self.device, self.head_dim
+        T, H, q_rs = _rows(q, None, dim, self.dtype, device, "q")
+        b, cols, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
         if max_kv is None:
-            max_kv = table.shape[1] * self.page_size
+            max_kv = cols * self.page_size
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _rows(out, H, self.head_dim, self.dtype, self.device, "out")
-        _require(out.shape[0] == T, "out needs q's rows")
+            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        To, _, o_rs = _rows(out, H, dim, self.dtype, device, "out")
+        if To != T:
+            raise ValueError(f"out: {T} rows needed, got {To}")
         lib, c = native.load(), 1 if causal else 0
-        with _on_device(self.device):
-            need = lib.s2s_op_attn_paged_ws(self._ref, H, b, T, max_new, max_kv, c, window)
-            if need < 0:
-                native.check(int(need), "s2s_op_attn_paged_ws")
-            if need and workspace is None:
-                workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-            native.check(lib.s2s_op_attn_paged(native.stream_handle(), self._ref, q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), H, table.data_ptr(), table.shape[1],
-                                               kv_len.data_ptr(), native.ptr(cu), b, T, max_new, max_kv, self.head_dim ** -0.5 if scale is None else scale, c, window,
-                                               native.ptr(workspace), workspace.numel() * workspace.element_size() if workspace is not None else 0), "s2s_op_attn_paged")
+        with _on_device(device) as stream:
+            if workspace is None:
+                need = lib.s2s_op_attn_paged_ws(self._ref, H, b, T, max_new, max_kv, c, window)
+                if need < 0:
+                    native.check(int(need), "s2s_op_attn_paged_ws")
+                if need:
+                    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            elif workspace.device != device or not workspace.is_contiguous():
+                raise ValueError(f"workspace: contiguous on {device} needed")
+            ws, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            native.check(lib.s2s_op_attn_paged(stream, self._ref, q.data_ptr(), q_rs, out.data_ptr(), o_rs, H, table.data_ptr(), cols, kv_len.data_ptr(),
+                                               0 if cu is None else cu.data_ptr(), b, T, max_new, max_kv, dim ** -0.5 if scale is None else scale, c, window, ws, ws_bytes),
+                         "s2s_op_attn_paged")
         return out
