@@ -21,15 +21,20 @@ constexpr int KV_GROUP = 32;                     // channels of one position tha
 // the two halves, which is where a pair of 16-bit operands wants them.
 __device__ __forceinline__ unsigned code_nibble(int e) { return (unsigned)((e >> 1) + 4 * (e & 1)); }
 
+__device__ __forceinline__ unsigned and_or(unsigned w, unsigned mask, unsigned bits) {
+    unsigned r;       // one instruction where the second constant sits in a vector register; the compiler makes it two with literals
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+    return r;
+}
 // 8 codes -> code - 8 as float16, exact: 0x6400 | c is 1024 + c, 0x6400 | c << 4 is 1024 + 16 c (both below 2048: no rounding)
 __device__ __forceinline__ void codes_to_f16(unsigned w, f16x2_t (&c)[4]) {
     const f16x2_t off = {(_Float16)-1032.f, (_Float16)-1032.f};
     const f16x2_t sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, off16 = {(_Float16)-72.f, (_Float16)-72.f};
     const unsigned w8 = w >> 8;
-    c[0] = __builtin_bit_cast(f16x2_t, (w & 0x000f000fu) | 0x64006400u) + off;
-    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (w & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
-    c[2] = __builtin_bit_cast(f16x2_t, (w8 & 0x000f000fu) | 0x64006400u) + off;
-    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, (w8 & 0x00f000f0u) | 0x64006400u), sixteenth, off16);
+    c[0] = __builtin_bit_cast(f16x2_t, and_or(w, 0x000f000fu, 0x64006400u)) + off;
+    c[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, and_or(w, 0x00f000f0u, 0x64006400u)), sixteenth, off16);
+    c[2] = __builtin_bit_cast(f16x2_t, and_or(w8, 0x000f000fu, 0x64006400u)) + off;
+    c[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, and_or(w8, 0x00f000f0u, 0x64006400u)), sixteenth, off16);
 }
 
 // fields of a packed cache handle, checked by paged_check (paged.hip)

@@ -174,8 +174,8 @@ template <typename V> __device__ __forceinline__ V ld_at(const void* base, unsig
 template <int KIND, int D> struct KeyTile {       // bf16, f32: octets of the U x 2 rows this lane stands for
     static constexpr int U = tile_u(KIND, D), EB = KIND == KV_F32 ? 4 : 2;
     typename KvT<KIND>::frag_t f[U][2][D / 32];
-    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return (((l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8) * EB; }
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+    static __device__ __forceinline__ unsigned lane_off(int, int l15, int g) { return (((l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8) * EB; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, int) {
         const char* base = (const char*)p.kc + ((head << p.r.ps_log2) + at) * D * EB;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -184,82 +184,99 @@ template <int KIND, int D> struct KeyTile {       // bf16, f32: octets of the U 
 #pragma unroll
                 for (int s = 0; s < D / 32; ++s) f[u][t][s] = ld_at<typename KvT<KIND>::frag_t>(base + ((u * 8 + t * 4) * D + s * 32) * EB, off);
     }
-    __device__ __forceinline__ typename KvT<KIND>::frag_t get(int u, int t, int s) const { return f[u][t][s]; }
+    __device__ __forceinline__ void ready(unsigned char*, int) {}
+    __device__ __forceinline__ typename KvT<KIND>::frag_t get(const unsigned char*, int, int, int u, int t, int s) const { return f[u][t][s]; }
 };
 template <int KIND, int D> struct ValTile {
     static constexpr int U = tile_u(KIND, D), EB = KIND == KV_F32 ? 4 : 2;
     typename KvT<KIND>::frag_t f[D / 16][U];
     static __device__ __forceinline__ unsigned lane_off(int l15, int g, int ps_log2) { return ((l15 << ps_log2) + g * 8 * U) * EB; }
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+    static __device__ __forceinline__ unsigned meta_off(int, int) { return 0; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, unsigned) {
         const char* base = (const char*)p.vc + (((head * D) << p.r.ps_log2) + at) * EB;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
 #pragma unroll
             for (int u = 0; u < U; ++u) f[d][u] = ld_at<typename KvT<KIND>::frag_t>(base + ((d * 16 << p.r.ps_log2) + u * 8) * EB, off);
     }
-    __device__ __forceinline__ void mask(int pos, int lo, int hi) {
+    // edge: values outside [lo, hi) become 0
+    __device__ __forceinline__ void ready(unsigned char*, int, int g, bool edge, int kb, int lo, int hi) {
+        if (!edge) return;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const OctetBits<typename KvT<KIND>::frag_t> bits(pos + u * 8, lo, hi);
+            const OctetBits<typename KvT<KIND>::frag_t> bits(kb + (g * U + u) * 8, lo, hi);
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) f[d][u] = bits.keep(f[d][u]);
         }
     }
-    __device__ __forceinline__ typename KvT<KIND>::frag_t get(int d, int u) const { return f[d][u]; }
+    __device__ __forceinline__ typename KvT<KIND>::frag_t get(const unsigned char*, int, int d, int u) const { return f[d][u]; }
+};
+// 4 bits: a lane needs the scales and zeros of its key rows (shared by 4 lanes) and of its 8 U positions in every group (shared by 16).  Loaded as
+// needed they would be two thirds of the lane traffic, and 80 registers at 128 channels; so the wave loads a tile's scales and zeros once, 8 or 16 bytes a
+// lane, and deals them out through LDS of its own.
+template <int D> struct CodeMeta {
+    static constexpr int U = tile_u(KV_INT4, D), TK = 32 * U, NS = D / 32, W = TK * NS / 64;      // dwords per lane; 64 lanes: a tile's keys or values
+    static constexpr int BYTES = W * 4 * 64;
+    typedef unsigned words_t __attribute__((ext_vector_type(W)));
 };
 template <int D> struct KeyTile<KV_INT4, D> {
-    static constexpr int U = tile_u(KV_INT4, D), NS = D / 32;
+    typedef CodeMeta<D> M;
+    static constexpr int U = M::U, NS = M::NS;
     typedef unsigned words_t __attribute__((ext_vector_type(NS)));
-    words_t w[U][2], m[U][2];
-    // codes at `off`, scales and zeros at off / D * 8: rows are D / 2 and D / 8 bytes
-    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return ((l15 >> 2) * 8 * U + (l15 & 3)) * (D / 2) + g * NS * 4; }
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+    words_t w[U][2];
+    typename M::words_t m;
+    static __device__ __forceinline__ unsigned lane_off(int, int l15, int g) { return ((l15 >> 2) * 8 * U + (l15 & 3)) * (D / 2) + g * NS * 4; }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, int lane) {
         const long row = (head << p.r.ps_log2) + at;
         const char* base = (const char*)p.kc + row * (D / 2);
-        const char* meta = (const char*)p.km + row * (D / 8);
-        const unsigned moff = off / (D / 2) * (D / 8);
+        m = ld_at<typename M::words_t>((const char*)p.km + row * (D / 8), lane * M::W * 4);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                w[u][t] = ld_at<words_t>(base + (u * 8 + t * 4) * (D / 2), off);
-                m[u][t] = ld_at<words_t>(meta + (u * 8 + t * 4) * (D / 8), moff);
-            }
+            for (int t = 0; t < 2; ++t) w[u][t] = ld_at<words_t>(base + (u * 8 + t * 4) * (D / 2), off);
     }
-    __device__ __forceinline__ f16x8_t get(int u, int t, int s) const { return dequant_key(w[u][t][s], m[u][t][s]); }
+    __device__ __forceinline__ void ready(unsigned char* own, int lane) {
+        __builtin_amdgcn_wave_barrier();           // the wave's reads of the last tile come first (LDS keeps a wave's order; the compiler must)
+        *reinterpret_cast<typename M::words_t*>(own + lane * M::W * 4) = m;
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ f16x8_t get(const unsigned char* own, int l15, int, int u, int t, int s) const {
+        const words_t row = *reinterpret_cast<const words_t*>(own + ((l15 >> 2) * 8 * U + (l15 & 3) + u * 8 + t * 4) * (D / 8));
+        return dequant_key(w[u][t][s], row[s]);
+    }
 };
 template <int D> struct ValTile<KV_INT4, D> {
-    static constexpr int U = tile_u(KV_INT4, D);
+    typedef CodeMeta<D> M;
+    static constexpr int U = M::U;
     typedef unsigned words_t __attribute__((ext_vector_type(U)));
     words_t w[D / 16];
-    f16x8_t s[D / 32][U], z[D / 32][U];
+    typename M::words_t m;
     static __device__ __forceinline__ unsigned lane_off(int l15, int g, int ps_log2) { return (l15 << (ps_log2 - 1)) + g * U * 4; }
-    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off) {
+    static __device__ __forceinline__ unsigned meta_off(int lane, int ps_log2) {                  // rows of TK float16: scales, zeros of every group
+        return (((unsigned)(lane * M::W * 2 / M::TK) << ps_log2) + lane * M::W * 2 % M::TK) * 2;
+    }
+    __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, unsigned moff) {
         const char* base = (const char*)p.vc + ((head * D) << (p.r.ps_log2 - 1)) + (at >> 1);
-        const _Float16* meta = p.vm + ((head * (D / 32) * 2) << p.r.ps_log2) + at;
-        const unsigned moff = (off & 31) * 4;      // g * 8 U positions of 2 bytes (a channel's row is a multiple of 32 bytes)
+        m = ld_at<typename M::words_t>((const char*)(p.vm + ((head * (D / 32) * 2) << p.r.ps_log2) + at), moff);
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) w[d] = ld_at<words_t>(base + (d * 16 << (p.r.ps_log2 - 1)), off);
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                s[k][u] = ld_at<f16x8_t>(meta + ((2 * k) << p.r.ps_log2) + u * 8, moff);
-                z[k][u] = ld_at<f16x8_t>(meta + ((2 * k + 1) << p.r.ps_log2) + u * 8, moff);
-            }
     }
-    __device__ __forceinline__ void mask(int pos, int lo, int hi) {     // scale and zero 0: a value of 0 whatever the code
+    // edge: scale and zero 0 outside [lo, hi), a value of 0 whatever the code
+    __device__ __forceinline__ void ready(unsigned char* own, int lane, int, bool edge, int kb, int lo, int hi) {
+        if (edge) {
+            const int first = kb + lane * M::W * 2 % M::TK;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const OctetBits<f16x8_t> bits(pos + u * 8, lo, hi);
-#pragma unroll
-            for (int k = 0; k < D / 32; ++k) {
-                s[k][u] = bits.keep(s[k][u]);
-                z[k][u] = bits.keep(z[k][u]);
-            }
+            for (int i = 0; i < M::W; ++i)
+                m[i] &= (first + 2 * i >= lo && first + 2 * i < hi ? 0xffffu : 0u) | (first + 2 * i + 1 >= lo && first + 2 * i + 1 < hi ? 0xffff0000u : 0u);
         }
+        __builtin_amdgcn_wave_barrier();
+        *reinterpret_cast<typename M::words_t*>(own + M::BYTES + lane * M::W * 4) = m;
+        __builtin_amdgcn_wave_barrier();
     }
-    __device__ __forceinline__ f16x8_t get(int d, int u) const { return dequant_val(w[d][u], s[d >> 1][u], z[d >> 1][u]); }
+    __device__ __forceinline__ f16x8_t get(const unsigned char* own, int g, int d, int u) const {
+        const unsigned char* row = own + M::BYTES + ((d >> 1) * 2 * M::TK + (g * U + u) * 8) * 2;
+        return dequant_val(w[d][u], *reinterpret_cast<const f16x8_t*>(row), *reinterpret_cast<const f16x8_t*>(row + M::TK * 2));
+    }
 };
 
 // 4 neighbouring channels of an output row
@@ -310,7 +327,7 @@ __device__ __forceinline__ float max_over_groups(float x) {        // over the 4
 
 // scores of a tile -> softmax step and products with the tile's values
 template <int KIND, int D>
-__device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2], const ValTile<KIND, D>& vt, float sc, float& m, float& l, f32x4_t (&acc)[D / 16]) {
+__device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2], const ValTile<KIND, D>& vt, const unsigned char* own, int g, float sc, float& m, float& l, f32x4_t (&acc)[D / 16]) {
     typedef typename KvT<KIND>::frag_t frag_t;
     constexpr int U = tile_u(KIND, D), ND = D / 16;
     float x[U][8], mx = NO_MAX;
@@ -355,7 +372,7 @@ __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2]
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            const frag_t v = vt.get(d, u);
+            const frag_t v = vt.get(own, g, d, u);
             acc[d] = mma(v, ph[u], acc[d]);
             if constexpr (KIND == KV_BF16) acc[d] = mma(v, pl[u], acc[d]);
         }
@@ -367,13 +384,15 @@ __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2]
 // by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
 // the next values behind this tile's products, so both are in flight while the other is used.
 template <int KIND, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND>::frag_t frag_t;
     constexpr int U = tile_u(KIND, D), TK = 32 * U, NS = D / 32, ND = D / 16;
     __shared__ float so[2][16][D + 4];
     __shared__ float sm[4][16], sl[4][16];
+    __shared__ alignas(16) unsigned char meta[KIND == KV_INT4 ? 4 * 2 * CodeMeta<D>::BYTES : 16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+    unsigned char* own = meta + (KIND == KV_INT4 ? wave * 2 * CodeMeta<D>::BYTES : 0);
     const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
     Span sp;
     if (!tile_span(p, b, vr0, 16, sp)) return;
@@ -398,12 +417,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
         KeyTile<KIND, D> kt;
         ValTile<KIND, D> vt;
         const int ps_mask = (1 << p.r.ps_log2) - 1;
-        const unsigned k_off = KeyTile<KIND, D>::lane_off(l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
+        const unsigned k_off = KeyTile<KIND, D>::lane_off(lane, l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
+        const unsigned m_off = ValTile<KIND, D>::meta_off(lane, p.r.ps_log2);
         int page = page_raw(p.r, b, kb), next = kb + 4 * TK < k1 ? page_raw(p.r, b, kb + 4 * TK) : -1;
         {
             const long head = (long)(page_ok(p.r, page) ? page : 0) * p.r.Hkv + hk;
-            kt.load(p, head, kb & ps_mask, k_off);
-            vt.load(p, head, kb & ps_mask, v_off);
+            kt.load(p, head, kb & ps_mask, k_off, lane);
+            vt.load(p, head, kb & ps_mask, v_off, m_off);
         }
         for (; kb < k1; kb += 4 * TK) {
             const int nb = kb + 4 * TK;
@@ -411,28 +431,30 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attn_paged_step_kernel(
             const int after = nb + 4 * TK < k1 ? page_raw(p.r, b, nb + 4 * TK) : -1;
             const int nat = nb < k1 ? nb & ps_mask : 0;
             f32x4_t s[U][2];
+            kt.ready(own, lane);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     s[u][tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < NS; ++k) s[u][tt] = mma(kt.get(u, tt, k), q[k], s[u][tt]);
+                    for (int k = 0; k < NS; ++k) s[u][tt] = mma(kt.get(own, l15, g, u, tt, k), q[k], s[u][tt]);
                 }
-            if (nb < k1) kt.load(p, nhead, nat, k_off);
+            if (nb < k1) kt.load(p, nhead, nat, k_off, lane);
             if (page_ok(p.r, page)) {
-                if (kb < sp.lo_all || kb + TK > sp.hi_all) {
+                const bool edge = kb < sp.lo_all || kb + TK > sp.hi_all;
+                if (edge) {
                     const int pos = kb + g * 8 * U;
 #pragma unroll
                     for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             if (pos + u * 8 + e < c_lo || pos + u * 8 + e >= c_hi) s[u][e >> 2][e & 3] = -INFINITY;
-                    vt.mask(pos, sp.lo, sp.hi);
                 }
-                step_tile<KIND, D>(s, vt, sc, m, l, acc);
+                vt.ready(own, lane, g, edge, kb, sp.lo, sp.hi);
+                step_tile<KIND, D>(s, vt, own, g, sc, m, l, acc);
             }
-            if (nb < k1) vt.load(p, nhead, nat, v_off);
+            if (nb < k1) vt.load(p, nhead, nat, v_off, m_off);
             page = next;
             next = after;
         }
@@ -491,43 +513,48 @@ template <int KIND, int D> struct LdsTile {
     static constexpr int U = tile_u(KIND, D), TK = 32 * U;
     static constexpr int EB = KIND == KV_F32 ? 4 : 2, OB = 8 * EB;  // bytes per element and per octet in LDS
     static constexpr int K_BYTES = TK * D * EB, BYTES = 2 * K_BYTES;
-    static constexpr int FB = U == 2 ? 4 : 3;                      // position bit that is bit 2 of its f
-    static __device__ __forceinline__ int kf(int key) { return (key & 3) | ((key >> FB) & 1) << 2; }
-    static __device__ __forceinline__ int vf(int d) { return d & (TK / 8 - 1); }
+    static constexpr int FB = U == 2 ? 4 : 3;                      // position bit that l15's bit 2 is
+    static constexpr int HB = D == 64 ? 1 : 2;                     // bits of f above the lowest two
+    // 16 lanes read together and the banks span 256 bytes: a key row of 128 channels or more takes all 16 of f, two rows of 64 share the span (the row's
+    // parity is the slot's top bit) and take 8
+    static __device__ __forceinline__ int kf(int key) { return D == 64 ? ((key >> 1) & 1) | ((key >> FB) & 3) << 1 : (key & 3) | ((key >> FB) & 3) << 2; }
+    static __device__ __forceinline__ int vf(int d) { return U == 2 ? (d >> 1) & 7 : KIND == KV_F32 ? d & 3 : (d >> 2) & 3; }
+    // value octets trade places so that lanes of neighbouring g, which share a read cycle on opposite quarters of the rows, stay apart too
+    static __device__ __forceinline__ int vs(int o) { return U == 2 ? (o & 1) << 2 | o >> 1 : KIND == KV_F32 ? o : (0x9c >> (2 * o)) & 3; }
+    static __device__ __forceinline__ int vo(int s) { return U == 2 ? (s & 3) << 1 | s >> 2 : KIND == KV_F32 ? s : (0x78 >> (2 * s)) & 3; }     // back
     static __device__ __forceinline__ int k_at(int key, int o) { return (key * (D / 8) + (o ^ kf(key))) * OB; }
-    static __device__ __forceinline__ int v_at(int d, int o) { return K_BYTES + (d * (TK / 8) + (o ^ vf(d))) * OB; }
+    static __device__ __forceinline__ int v_at(int d, int o) { return K_BYTES + (d * (TK / 8) + (vs(o) ^ vf(d))) * OB; }
 };
-// The reading side: f of a lane's key rows is l15 % 8 and of its value rows l15 % (TK / 8), whatever the product, so four lane offsets serve all reads
-// and the rest are constants: octet 4 k + g of a key row lies 4 OB (k ^ f / 4) behind octet (g ^ f % 4).
+// The reading side: f depends on l15 only, whatever the product, so a few lane offsets serve all reads and the rest are constants: octet 4 k + g of a key
+// row lies 4 OB (k ^ f / 4) behind octet (g ^ f % 4).
 template <int KIND, int D> struct LdsOff {
     typedef LdsTile<KIND, D> L;
-    int k[2], v[L::U];
+    static constexpr int NK = 1 << L::HB;
+    int k[NK], v[L::U];
     __device__ __forceinline__ LdsOff(int l15, int g) {
         const int key = (l15 >> 2) * 8 * L::U + (l15 & 3);
-        k[0] = L::k_at(key, g);                    // even k: + 4 OB k
-        k[1] = L::k_at(key, 4 + g) - 4 * L::OB;    // odd k: + 4 OB k
+#pragma unroll
+        for (int i = 0; i < NK; ++i) k[i] = L::k_at(key, 4 * i + g) - 4 * L::OB * i;
 #pragma unroll
         for (int u = 0; u < L::U; ++u) v[u] = L::v_at(l15, g * L::U + u);
     }
 };
 
-// page -> LDS: 16-byte pieces in LDS order, the swizzle in the lane's source offset (which changes with the piece only by f's bit 2)
+// page -> LDS: 16-byte pieces in LDS order, the swizzle in the lane's source offset (a piece further on in the tile changes only the bits of f that come
+// from the position bits its step reaches)
 template <int KIND, int D> struct TileDma {
     typedef LdsTile<KIND, D> L;
     static constexpr int PB = L::EB / 2;                           // pieces per octet
     static constexpr int N = L::K_BYTES / 16 / 256;                // pieces per thread, keys or values
     static constexpr int KS = 256 / PB / (D / 8);                  // key rows per piece of the workgroup
     static constexpr int VS = 256 / PB / (L::TK / 8);              // value rows
-    unsigned k[2], v;
+    unsigned k[N], v;
     __device__ __forceinline__ TileDma(int tid, int ps_log2) {
         const int o = tid / PB, half = tid % PB;
         const int key = o / (D / 8), d = o / (L::TK / 8);
 #pragma unroll
-        for (int bit = 0; bit < 2; ++bit) {
-            const int f = (key & 3) | (KS > (1 << L::FB) ? (key >> L::FB) & 1 : bit) << 2;
-            k[bit] = (key * D + ((o % (D / 8)) ^ f) * 8) * L::EB + half * 16;
-        }
-        v = (((unsigned)d << ps_log2) + ((o % (L::TK / 8)) ^ L::vf(d)) * 8) * L::EB + half * 16;
+        for (int i = 0; i < N; ++i) k[i] = (key * D + ((o % (D / 8)) ^ L::kf(i * KS + key)) * 8) * L::EB + half * 16;
+        v = (((unsigned)d << ps_log2) + L::vo((o % (L::TK / 8)) ^ L::vf(d)) * 8) * L::EB + half * 16;
     }
     __device__ __forceinline__ void start(const PagedAttn& p, unsigned char* buf, int page, int hk, int at, int wave) const {
         const long head = (long)page * p.r.Hkv + hk;
@@ -535,7 +562,7 @@ template <int KIND, int D> struct TileDma {
         const char* vb = (const char*)p.vc + (((head * D) << p.r.ps_log2) + at) * L::EB;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + i * KS * D * L::EB + k[((i * KS) >> L::FB) & 1]),
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + i * KS * D * L::EB + k[i]),
                                              (__attribute__((address_space(3))) void*)(buf + (i * 4 + wave) * 1024), 16, 0, 0);
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -576,80 +603,90 @@ template <int D> struct CodeRegs {
     }
 };
 
-// one tile: scores, softmax step, products with the values, 32 positions at a time
+// one tile: scores, softmax step, products with the values
 template <int KIND, int D, int NC>
 __device__ __forceinline__ void tile_step(const unsigned char* buf, const LdsOff<KIND, D>& off, const typename KvT<KIND>::frag_t (&q)[NC][D / 32], const float (&sc)[NC],
                                           bool edge, int pos0, const int (&c_lo)[NC], const int (&c_hi)[NC], float (&m)[NC], float (&l)[NC], f32x4_t (&acc)[NC][D / 16]) {
     typedef typename KvT<KIND>::frag_t frag_t;
     typedef LdsTile<KIND, D> L;
     constexpr int U = L::U, NS = D / 32, ND = D / 16;
+    f32x4_t s[NC][U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int pos = pos0 + u * 8;
-        f32x4_t s[NC][2];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[c][0] = s[c][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
-            for (int k = 0; k < NS; ++k) {
-                const frag_t a = *reinterpret_cast<const frag_t*>(buf + off.k[k & 1] + ((u * 8 + tt * 4) * (D / 8) + 4 * k) * L::OB);
+            for (int c = 0; c < NC; ++c) s[c][u][tt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < NC; ++c) s[c][tt] = mma(a, q[c][k], s[c][tt]);
+            for (int k = 0; k < NS; ++k) {
+                const frag_t a = *reinterpret_cast<const frag_t*>(buf + off.k[k & (LdsOff<KIND, D>::NK - 1)] + ((u * 8 + tt * 4) * (D / 8) + 4 * k) * L::OB);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) s[c][u][tt] = mma(a, q[c][k], s[c][u][tt]);
             }
         }
-        if (edge) {
+    if (edge) {
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (pos + e < c_lo[c] || pos + e >= c_hi[c]) s[c][e >> 2][e & 3] = -INFINITY;
-        }
-        float x[NC][8];
-        bool raise = false;
+                    if (pos0 + u * 8 + e < c_lo[c] || pos0 + u * 8 + e >= c_hi[c]) s[c][u][e >> 2][e & 3] = -INFINITY;
+    }
+    float x[NC][U][8];
+    bool raise = false;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            float mx = NO_MAX;
+    for (int c = 0; c < NC; ++c) {
+        float mx = NO_MAX;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -m[c]);
-                mx = fmaxf(mx, x[c][e]);
-            }
-            raise |= mx > MAX_SLACK;
-        }
-        if (__any(raise)) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float mn = m[c];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[c][e >> 2][e & 3] * sc[c]);
-                mn = max_over_groups(mn);
-                const float a = __builtin_amdgcn_exp2f(m[c] - mn);
-                m[c] = mn;
-                l[c] *= a;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) acc[c][d] *= a;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e] = fmaf(s[c][e >> 2][e & 3], sc[c], -mn);
-            }
-        }
-        frag_t pr[NC];
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[c][e] = __builtin_amdgcn_exp2f(x[c][e]);
-                l[c] += x[c][e];
+                x[c][u][e] = fmaf(s[c][u][e >> 2][e & 3], sc[c], -m[c]);
+                mx = fmaxf(mx, x[c][u][e]);
             }
-            probs(x[c], pr[c]);
+        raise |= mx > MAX_SLACK;
+    }
+    if (__any(raise)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            float mn = m[c];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[c][u][e >> 2][e & 3] * sc[c]);
+            mn = max_over_groups(mn);
+            const float a = __builtin_amdgcn_exp2f(m[c] - mn);
+            m[c] = mn;
+            l[c] *= a;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) acc[c][d] *= a;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][u][e] = fmaf(s[c][u][e >> 2][e & 3], sc[c], -mn);
         }
+    }
+    frag_t pr[NC][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[c][u][e] = __builtin_amdgcn_exp2f(x[c][u][e]);
+                l[c] += x[c][u][e];
+            }
+            probs(x[c][u], pr[c][u]);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             const frag_t v = *reinterpret_cast<const frag_t*>(buf + off.v[u] + d * 16 * (L::TK / 8) * L::OB);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) acc[c][d] = mma(v, pr[c], acc[c][d]);
+            for (int c = 0; c < NC; ++c) acc[c][d] = mma(v, pr[c][u], acc[c][d]);
         }
-    }
 }
 
 template <int KIND, int D, int NC>
@@ -697,43 +734,41 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
     }
 
     const int ps_mask = (1 << p.r.ps_log2) - 1;
-    int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, cur = 0;
-    int next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1;
+    int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1, cur = 0;
     CodeRegs<D> regs;
     const LdsOff<KIND, D> off(l15, g);
     const TileDma<KIND == KV_INT4 ? KV_BF16 : KIND, D> dma(tid, p.r.ps_log2);
-    if constexpr (KIND == KV_INT4) {
+    if constexpr (KIND == KV_INT4) {               // codes of tile t + 1 are in registers when tile t is begun
         if (page_ok(p.r, page)) {
             regs.load(p, page, hk, k0 & ps_mask, tid);
             regs.store(lds, tid);
         }
         if (page_ok(p.r, next)) regs.load(p, next, hk, (k0 + TK) & ps_mask, tid);
-    } else {
-        if (page_ok(p.r, page)) dma.start(p, lds, page, hk, k0 & ps_mask, wave);
+    } else if (page_ok(p.r, page)) {
+        dma.start(p, lds, page, hk, k0 & ps_mask, wave);
     }
     for (int kb = k0; kb < k1; kb += TK) {
         __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed
         __builtin_amdgcn_s_barrier();              // everyone's has, and everyone is done with the other buffer
-        const unsigned char* buf = lds + cur * L::BYTES;
+        unsigned char* buf = lds + cur * L::BYTES;
         unsigned char* other = lds + (cur ^ 1) * L::BYTES;
         const int after = kb + 2 * TK < k1 ? page_raw(p.r, b, kb + 2 * TK) : -1;
         if constexpr (KIND == KV_INT4) {
             if (page_ok(p.r, next)) regs.store(other, tid);
             if (page_ok(p.r, after)) regs.load(p, after, hk, (kb + 2 * TK) & ps_mask, tid);
-        } else {
-            if (page_ok(p.r, next)) dma.start(p, other, next, hk, (kb + TK) & ps_mask, wave);
+        } else if (page_ok(p.r, next)) {
+            dma.start(p, other, next, hk, (kb + TK) & ps_mask, wave);
         }
         if (kb < sp.lo || kb + TK > sp.hi) {       // the first and last tile: values nobody attends to become 0 where they lie
             for (int i = tid; i < D * TK / 8; i += 256) {
                 const int d = i / (TK / 8), o = i % (TK / 8);
-                frag_t* v = reinterpret_cast<frag_t*>(lds + cur * L::BYTES + L::v_at(d, o));
+                frag_t* v = reinterpret_cast<frag_t*>(buf + L::v_at(d, o));
                 *v = OctetBits<frag_t>(kb + o * 8, sp.lo, sp.hi).keep(*v);
             }
             __syncthreads();
         }
-        if (page_ok(p.r, page) && kb < sw.hi && kb + TK > sw.lo) {
+        if (page_ok(p.r, page) && kb < sw.hi && kb + TK > sw.lo)
             tile_step<KIND, D, NC>(buf, off, q, sc, kb < sw.lo_all || kb + TK > sw.hi_all, kb + g * 8 * U, c_lo, c_hi, m, l, acc);
-        }
         page = next;
         next = after;
         cur ^= 1;
@@ -762,31 +797,45 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
     }
 }
 
-// ---- the splits' partial results of one (row, head) -> its output: a wave each, in split order -----------------------------------------------
-template <typename T, int D>
+// ---- the splits' partial results of one (row, head) -> its output -------------------------------------------------------------------------------
+// WAVES waves each: wave w adds the splits w, w + WAVES, ... in order, the sums meet in LDS.  Bound by the latency of its loads where there are many splits
+// (4 waves), by their bytes where there are many rows (one wave, 4 rows a workgroup).
+template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn p) {
     constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6), n = (long)p.r.T * p.H;
+    __shared__ float so[WAVES == 4 ? 3 : 1][D], sl[4];
+    typedef float vec_t __attribute__((ext_vector_type(E)));
+    const int lane = threadIdx.x & 63, wave = WAVES == 4 ? threadIdx.x >> 6 : 0;
+    const long n = (long)p.r.T * p.H, i = WAVES == 4 ? blockIdx.x : (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= n) return;
     const int row = (int)(i / p.H), h = (int)(i - (long)row * p.H);
     if (p.r.cu && (row < p.r.cu[0] || row >= p.r.cu[p.r.B])) return;
-    float M = -INFINITY;
+    float M = NO_MAX;
     for (int s = lane; s < p.n_splits; s += 64) M = fmaxf(M, p.plse[s * n + i]);
     M = wave_max(M);
     float acc[E], L = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    const float Ms = M == -INFINITY ? 0.f : M;
 #pragma unroll 4
-    for (int s = 0; s < p.n_splits; ++s) {
+    for (int s = wave; s < p.n_splits; s += WAVES) {
         const float lse = p.plse[s * n + i];
         if (lse == -INFINITY) continue;     // nothing was written for it
-        const float w = __builtin_amdgcn_exp2f(lse - Ms);
+        const float w = __builtin_amdgcn_exp2f(lse - M);
         L += w;
-        const float* src = p.po + (s * n + i) * D + lane * E;
+        const vec_t v = *reinterpret_cast<const vec_t*>(p.po + (s * n + i) * D + lane * E);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, src[e], acc[e]);
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(w, ((const float*)&v)[e], acc[e]);
+    }
+    if constexpr (WAVES == 4) {
+        if (lane == 0) sl[wave] = L;
+        if (wave)
+#pragma unroll
+            for (int e = 0; e < E; ++e) so[wave - 1][lane * E + e] = acc[e];
+        __syncthreads();
+        if (wave) return;
+        L = sl[0] + sl[1] + sl[2] + sl[3];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += so[0][lane * E + e] + so[1][lane * E + e] + so[2][lane * E + e];
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
     T* o = (T*)p.o + row * p.o_rs + (long)h * D + lane * E;
@@ -809,7 +858,7 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
     pl.q_tiles = cdiv((long)max_new * G, rows);
     const long span = causal && window > 0 ? std::min<long>(max_kv, (long)window + cdiv(rows - 1, G) + 1 + 63) + 63 : max_kv;      // from a multiple of 64
     const long groups = (long)B * kv->kv_heads * pl.q_tiles;
-    const long want = std::max<long>(1, 1024 / std::max<long>(1, groups));
+    const long want = std::max<long>(1, (pl.tile ? 512 : 1024) / std::max<long>(1, groups));
     pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
     pl.n_splits = std::max(1, cdiv(span, pl.chunk));
     if (pl.n_splits == 1) pl.chunk = 1 << 30;
@@ -819,7 +868,8 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
     if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
     else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
-    if (p.n_splits > 1) attn_paged_join_kernel<T, D><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
+    if (p.n_splits > 8) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
+    else if (p.n_splits > 1) attn_paged_join_kernel<T, D, 1><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }
 
 }  // namespace s2s
