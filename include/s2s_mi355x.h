@@ -279,7 +279,7 @@ int32_t s2s_op_rope(void* stream, const void* x, int64_t x_rs, int64_t x_hs, voi
                     const float* cos_dev, const float* sin_dev, int32_t max_pos, int32_t rows, int32_t heads, int32_t head_dim, int32_t rotary_dim,
                     int32_t interleaved, int32_t dtype);
 
-/* Appends every session's new rows behind the start_dev[b] (int32, >= 0) positions its pages hold: the keys turned to their positions, the values as
+/* Appends every session's new rows behind the start_dev[b] (int32, 0 .. 2^30) positions its pages hold: the keys turned to their positions, the values as
  * they are.  cos_dev NULL: keys are stored as they come (rotary_dim ignored).  q (optional, H heads) is turned along into q_out (may be q). */
 int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, const void* k, int64_t k_rs, const void* v, int64_t v_rs, const void* q, int64_t q_rs,
                                void* q_out, int64_t qo_rs, int32_t H, const int32_t* table_dev, int32_t table_cols, const int32_t* start_dev,

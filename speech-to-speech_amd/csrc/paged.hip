@@ -116,82 +116,113 @@ __device__ __forceinline__ void turned_octet(const T* row, int o, const Turn& t,
     }
 }
 
-// One unit of NH heads of one row: the channels that turn together are read before any is written, so that out may be x.  The table's values stay
-// in registers over the heads.  VEC units: octet pairs (half layout: rot / 16) or octets (interleaved: rot / 8), then the octets that pass;
-// else channel pairs, then the channels that pass.
+// 16 bytes of a row: 8 bf16 or 4 f32
+template <typename T> struct Piece {
+    static constexpr int E = 16 / sizeof(T);
+    u32x4_t w;
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    }
+    __device__ __forceinline__ void put(const float (&y)[E]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(y[i]);
+            else w[i] = pack_bf16x2_hw(y[2 * i], y[2 * i + 1]);
+        }
+    }
+};
+
+// One unit of NH heads of one row: the channels that turn together are read before any is written, so that out may be x, and the table's values stay in
+// registers over the heads.  VEC units: half layout, two pieces, piece u and its partner half a rotation on; interleaved, one piece; then what passes, in
+// the same numbers of pieces and on the same path, so that lanes that turn and lanes that pass share their loads.  Else channel pairs, then single
+// channels that pass.
 template <typename T, bool VEC, int NH>
-__device__ __forceinline__ void turn_heads(const T* x, long x_hs, T* out, long o_hs, int heads, int u, const Turn& t, int pos) {
+__device__ __forceinline__ void turn_heads(const T* x, long x_hs, T* out, long o_hs, int heads, int u, const Turn& t, int pos, int D) {
     const int half = t.rot >> 1;
-    const int turning = VEC ? (t.inter ? t.rot >> 3 : t.rot >> 4) : half;
     const bool bad = pos >= t.max_pos;
     const float nan = __builtin_nanf("");
-    if (u >= turning) {            // passes
-        if (out == x) return;
-        const int d = VEC ? t.rot + 8 * (u - turning) : t.rot + (u - turning);
-#pragma unroll
-        for (int h = 0; h < NH; ++h)
-            if (h < heads) {
-                if constexpr (VEC) {
-                    Oct<T> a;
-                    oct_load<T, true>(a, x + h * x_hs + d);
-                    oct_store<T, true>(out + h * o_hs + d, a);
-                } else {
-                    out[h * o_hs + d] = x[h * x_hs + d];
-                }
-            }
-        return;
-    }
     const long tp = bad ? 0 : (long)pos * half;
     if constexpr (VEC) {
-        Oct<T> a[NH], b[NH];
+        constexpr int E = Piece<T>::E;
+        const int turning = t.inter ? t.rot / E : half / E;
+        const bool pass = u >= turning;
+        if (pass && out == x) return;
+        Piece<T> a[NH], b[NH];
         if (t.inter) {
-            const int d = 8 * u;
-            const float4 cc = *reinterpret_cast<const float4*>(t.cosT + tp + 4 * u), ss = *reinterpret_cast<const float4*>(t.sinT + tp + 4 * u);
-            const float cv[4] = {bad ? nan : cc.x, bad ? nan : cc.y, bad ? nan : cc.z, bad ? nan : cc.w}, sv[4] = {ss.x, ss.y, ss.z, ss.w};
+            const int d = E * u;
+            float cv[E / 2], sv[E / 2];
+#pragma unroll
+            for (int i = 0; i < E / 2; i += 2) {       // (a unit that passes reads the table's first entries)
+                const float2 c = *reinterpret_cast<const float2*>(t.cosT + tp + (pass ? 0 : d / 2) + i), s = *reinterpret_cast<const float2*>(t.sinT + tp + (pass ? 0 : d / 2) + i);
+                cv[i] = bad ? nan : c.x;
+                cv[i + 1] = bad ? nan : c.y;
+                sv[i] = s.x;
+                sv[i + 1] = s.y;
+            }
 #pragma unroll
             for (int h = 0; h < NH; ++h)
-                if (h < heads) oct_load<T, true>(a[h], x + h * x_hs + d);
+                if (h < heads) a[h].w = *reinterpret_cast<const u32x4_t*>(x + h * x_hs + d);
 #pragma unroll
             for (int h = 0; h < NH; ++h)
                 if (h < heads) {
-                    float y[8];
+                    float y[E];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = oct_get(a[h], 2 * i), q = oct_get(a[h], 2 * i + 1);
+                    for (int i = 0; i < E / 2; ++i) {
+                        const float p = a[h].get(2 * i), q = a[h].get(2 * i + 1);
                         y[2 * i] = turn_a(p, q, cv[i], sv[i]);
                         y[2 * i + 1] = turn_b(p, q, cv[i], sv[i]);
                     }
-                    oct_put(a[h], y);
-                    oct_store<T, true>(out + h * o_hs + d, a[h]);
+                    if (!pass) a[h].put(y);
+                    *reinterpret_cast<u32x4_t*>(out + h * o_hs + d) = a[h].w;
                 }
         } else {
-            const int d = 8 * u;
-            Oct<float> cc, ss;
-            oct_load<float, true>(cc, t.cosT + tp + d);
-            oct_load<float, true>(ss, t.sinT + tp + d);
+            const int d = pass ? t.rot + 2 * E * (u - turning) : E * u, d1 = pass ? min(d + E, D - E) : d + half, dt = pass ? 0 : d;
+            float cv[E], sv[E];
+#pragma unroll
+            for (int i = 0; i < E; i += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(t.cosT + tp + dt + i), s = *reinterpret_cast<const float4*>(t.sinT + tp + dt + i);
+                cv[i] = bad ? nan : c.x;
+                cv[i + 1] = bad ? nan : c.y;
+                cv[i + 2] = bad ? nan : c.z;
+                cv[i + 3] = bad ? nan : c.w;
+                sv[i] = s.x;
+                sv[i + 1] = s.y;
+                sv[i + 2] = s.z;
+                sv[i + 3] = s.w;
+            }
 #pragma unroll
             for (int h = 0; h < NH; ++h)
                 if (h < heads) {
-                    oct_load<T, true>(a[h], x + h * x_hs + d);
-                    oct_load<T, true>(b[h], x + h * x_hs + d + half);
+                    a[h].w = *reinterpret_cast<const u32x4_t*>(x + h * x_hs + d);
+                    b[h].w = *reinterpret_cast<const u32x4_t*>(x + h * x_hs + d1);
                 }
 #pragma unroll
             for (int h = 0; h < NH; ++h)
                 if (h < heads) {
-                    float ya[8], yb[8];
+                    float ya[E], yb[E];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float p = oct_get(a[h], i), q = oct_get(b[h], i), c = bad ? nan : oct_get(cc, i), s = oct_get(ss, i);
-                        ya[i] = turn_a(p, q, c, s);
-                        yb[i] = turn_b(p, q, c, s);
+                    for (int i = 0; i < E; ++i) {
+                        const float p = a[h].get(i), q = b[h].get(i);
+                        ya[i] = turn_a(p, q, cv[i], sv[i]);
+                        yb[i] = turn_b(p, q, cv[i], sv[i]);
                     }
-                    oct_put(a[h], ya);
-                    oct_put(b[h], yb);
-                    oct_store<T, true>(out + h * o_hs + d, a[h]);
-                    oct_store<T, true>(out + h * o_hs + d + half, b[h]);
+                    if (!pass) {
+                        a[h].put(ya);
+                        b[h].put(yb);
+                    }
+                    *reinterpret_cast<u32x4_t*>(out + h * o_hs + d) = a[h].w;
+                    *reinterpret_cast<u32x4_t*>(out + h * o_hs + d1) = b[h].w;
                 }
         }
     } else {
+        if (u >= half) {
+            const int d = t.rot + (u - half);
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+                if (h < heads) out[h * o_hs + d] = x[h * x_hs + d];
+            return;
+        }
         const int d0 = t.inter ? 2 * u : u, d1 = t.inter ? 2 * u + 1 : u + half;
         const float c = bad ? nan : t.cosT[tp + u], s = t.sinT[tp + u];
 #pragma unroll
@@ -203,8 +234,9 @@ __device__ __forceinline__ void turn_heads(const T* x, long x_hs, T* out, long o
             }
     }
 }
-inline int turn_units(bool vec, bool inter, int rot, int D) {
-    return vec ? (inter ? rot / 8 : rot / 16) + (D - rot) / 8 : rot / 2 + (D - rot);
+inline int turn_units(bool vec, bool inter, int rot, int D, int es) {
+    const int E = 16 / es;
+    return !vec ? rot / 2 + (D - rot) : inter ? D / E : rot / 2 / E + (D - rot + 2 * E - 1) / (2 * E);
 }
 
 struct RopeParams {
@@ -212,7 +244,7 @@ struct RopeParams {
     long x_rs, x_hs, o_rs, o_hs;
     const int* pos;
     Turn t;
-    int rows, heads, units;
+    int rows, heads, units, D;
 };
 template <typename T, bool VEC, int NH> __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
     const unsigned idx = blockIdx.x * 256u + threadIdx.x;
@@ -221,7 +253,7 @@ template <typename T, bool VEC, int NH> __global__ __launch_bounds__(256) void r
     const int pos = p.pos[r], h0 = blockIdx.y * NH;
     if (pos < 0) return;
     turn_heads<T, VEC, NH>((const T*)p.x + (long)r * p.x_rs + h0 * p.x_hs, p.x_hs, (T*)p.out + (long)r * p.o_rs + h0 * p.o_hs, p.o_hs, min(NH, p.heads - h0), (int)u, p.t,
-                           pos);
+                           pos, p.D);
 }
 
 // ---- 4-bit groups --------------------------------------------------------------------------------------------------------------------------
@@ -251,6 +283,7 @@ __device__ __forceinline__ unsigned code_of(float x, float scale, float zero) {
     if (!(scale > 0.f)) return 8u;
     return (unsigned)(fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, zero), scale)) + 8.f, 0.f), 15.f));
 }
+__device__ __forceinline__ float value_of(unsigned code, float scale, float zero) { return __fadd_rn(zero, __fmul_rn(scale, (float)code - 8.f)); }
 __device__ __forceinline__ unsigned meta_word(_Float16 scale, _Float16 zero) {
     return (unsigned)__builtin_bit_cast(unsigned short, scale) | (unsigned)__builtin_bit_cast(unsigned short, zero) << 16;
 }
@@ -378,7 +411,7 @@ __global__ __launch_bounds__(256) void kv_append_block_kernel(AppendParams p) {
             const int r = i / p.units, u = i - r * p.units;
             const T* src = (const T*)p.q + (src0 + r) * p.q_rs + (long)h0 * D;
             T* dst = (T*)p.qo + (src0 + r) * p.qo_rs + (long)h0 * D;
-            turn_heads<T, VEC, 4>(src, D, dst, D, min(4, p.H - h0), u, p.t, lo + r);
+            turn_heads<T, VEC, 4>(src, D, dst, D, min(4, p.H - h0), u, p.t, lo + r, D);
         }
         return;
     }
@@ -469,6 +502,21 @@ struct ReadParams {
     const int* start;
 };
 
+// key octet o of a page's row
+template <typename T, int KIND, int D> __device__ __forceinline__ void get_key(const ReadParams& p, long row, int o, Oct<T>& x) {
+    if constexpr (KIND != KV_INT4) {
+        oct_load<T, true>(x, (const T*)p.kc + row * D + 8 * o);
+    } else {
+        const int s = o >> 2, g = o & 3;
+        const unsigned w = reinterpret_cast<const unsigned*>(p.kc)[row * (D / 8) + g * (D / 32) + s];
+        const f16x2_t m = __builtin_bit_cast(f16x2_t, reinterpret_cast<const unsigned*>(p.km)[row * (D / 32) + s]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = value_of(w >> (4 * code_nibble(j)) & 15, (float)m[0], (float)m[1]);
+        oct_put(x, v);
+    }
+}
+
 // the same runs of 64 positions as the append; values go back through the LDS transpose
 template <typename T, int KIND, int D, bool VEC>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
@@ -495,15 +543,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (page < 0) {
                 oct_put(x, v);
-            } else if constexpr (KIND != KV_INT4) {
-                oct_load<T, true>(x, (const T*)p.kc + row * D + 8 * o);
             } else {
-                const int s = o >> 2, g = o & 3;
-                const unsigned w = reinterpret_cast<const unsigned*>(p.kc)[row * (D / 8) + g * (D / 32) + s];
-                const f16x2_t m = __builtin_bit_cast(f16x2_t, reinterpret_cast<const unsigned*>(p.km)[row * (D / 32) + s]);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __fadd_rn((float)m[1], __fmul_rn((float)m[0], (float)(w >> (4 * code_nibble(j)) & 15) - 8.f));
-                oct_put(x, v);
+                get_key<T, KIND, D>(p, row, o, x);
             }
             oct_store<T, VEC>((T*)p.ko + (dst0 + r) * p.o_rs + (long)y * D + 8 * o, x);
         }
@@ -528,7 +569,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
             const _Float16* m = p.vm + ((head * (D / 32) + (d0 + d) / 32) * 2 << p.r.ps_log2) + at0 + o * 8;
             const f16x8_t scale = *reinterpret_cast<const f16x8_t*>(m), zero = *reinterpret_cast<const f16x8_t*>(m + ((long)1 << p.r.ps_log2));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __fadd_rn((float)zero[j], __fmul_rn((float)scale[j], (float)(w >> (4 * code_nibble(j)) & 15) - 8.f));
+            for (int j = 0; j < 8; ++j) v[j] = value_of(w >> (4 * code_nibble(j)) & 15, (float)scale[j], (float)zero[j]);
             oct_put(x, v);
         }
         T e[8];
@@ -545,6 +586,42 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadParams p) {
         for (int w = 0; w < (int)sizeof(T) * 2; ++w) x.w[w >> 2][w & 3] = src[w];
         oct_store<T, VEC>((T*)p.vo + (dst0 + r) * p.o_rs + (long)h * D + d0 + 8 * o, x);
     }
+}
+
+// one position per session: D / 8 lanes per row of a head, values gathered channel by channel
+template <typename T, int KIND, int D, bool VEC>
+__global__ __launch_bounds__(256) void kv_read_step_kernel(ReadParams p) {
+    constexpr int LPT = D / 8;
+    const int b = blockIdx.y, task = (blockIdx.x * 256 + threadIdx.x) / LPT, o = threadIdx.x % LPT, Hkv = p.r.Hkv;
+    if (task >= 2 * Hkv || !(task < Hkv ? p.ko : p.vo)) return;
+    int row0, n;
+    session_rows(p.r, b, row0, n);
+    const int pos = p.start[b];
+    if (n <= 0 || row0 >= p.r.T || pos < 0 || pos > (1 << 30)) return;
+    const int page = page_of(p.r, b, pos), at = pos & ((1 << p.r.ps_log2) - 1), h = task < Hkv ? task : task - Hkv;
+    const long head = (long)max(page, 0) * Hkv + h;
+    Oct<T> x;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    oct_put(x, v);
+    if (page >= 0) {
+        if (task < Hkv) {
+            get_key<T, KIND, D>(p, (head << p.r.ps_log2) + at, o, x);
+        } else if constexpr (KIND != KV_INT4) {
+            T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = ((const T*)p.vc)[((head * D + 8 * o + i) << p.r.ps_log2) + at];
+            __builtin_memcpy(&x, e, sizeof(x));
+        } else {
+            const unsigned nib = code_nibble(at & 7);
+            const unsigned char* src = (const unsigned char*)p.vc + ((head * D + 8 * o) << (p.r.ps_log2 - 1)) + (at >> 3) * 4 + (nib >> 1);
+            const _Float16* m = p.vm + (((head * (D / 32) + (o >> 2)) * 2) << p.r.ps_log2) + at;
+            const float scale = m[0], zero = m[(long)1 << p.r.ps_log2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = value_of(src[(long)i << (p.r.ps_log2 - 1)] >> (nib & 1) * 4 & 15, scale, zero);
+            oct_put(x, v);
+        }
+    }
+    oct_store<T, VEC>((T*)(task < Hkv ? p.ko : p.vo) + (long)row0 * p.o_rs + (long)h * D + 8 * o, x);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------------------------------
@@ -609,6 +686,12 @@ static void append_launch(hipStream_t st, const AppendParams& p, bool vec) {
 
 template <typename T, int KIND, int D>
 static void read_launch(hipStream_t st, const ReadParams& p, bool vec) {
+    if (p.r.max_new == 1) {
+        const dim3 grid(cdiv(2L * p.r.Hkv * (D / 8), 256), p.r.B);
+        if (vec) kv_read_step_kernel<T, KIND, D, true><<<grid, 256, 0, st>>>(p);
+        else kv_read_step_kernel<T, KIND, D, false><<<grid, 256, 0, st>>>(p);
+        return;
+    }
     const dim3 grid(cdiv((long)p.r.max_new + 63, 64), p.r.Hkv + p.r.Hkv * (D / 64), p.r.B);
     if (vec) kv_read_kernel<T, KIND, D, true><<<grid, 256, 0, st>>>(p);
     else kv_read_kernel<T, KIND, D, false><<<grid, 256, 0, st>>>(p);
@@ -632,7 +715,7 @@ extern "C" int32_t s2s_op_rope(void* stream, const void* x, int64_t x_rs, int64_
     const bool vec = rotary_dim % 16 == 0 && head_dim % 8 == 0 && aligned(x, x_rs, es) && aligned(out, o_rs, es) && (x_hs * es) % 16 == 0 && (o_hs * es) % 16 == 0 &&
                      aligned(cos_dev, 0, 4) && aligned(sin_dev, 0, 4);
     RopeParams p{x, out, x_rs, x_hs, o_rs, o_hs, positions_dev, Turn{cos_dev, sin_dev, max_pos, rotary_dim, interleaved != 0}, rows, heads,
-                 turn_units(vec, interleaved != 0, rotary_dim, head_dim)};
+                 turn_units(vec, interleaved != 0, rotary_dim, head_dim, es), head_dim};
     S2S_REQUIRE((long)rows * p.units < (1L << 31), "rope: %d rows of %d units are too many for one call", rows, p.units);
     const bool many = (long)rows * p.units * heads >= 256L * 1024 * 4;     // enough for every CU with 4 heads a thread
     if (dtype == S2S_F32) {
@@ -669,7 +752,7 @@ extern "C" int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, 
     p.k = k; p.k_rs = k_rs; p.v = v; p.v_rs = v_rs; p.q = q; p.q_rs = q_rs; p.qo = q_out; p.qo_rs = qo_rs;
     p.start = start_dev;
     p.H = q ? H : 0;
-    p.units = q ? turn_units(vec, p.t.inter, p.t.rot, kv->head_dim) : 1;
+    p.units = q ? turn_units(vec, p.t.inter, p.t.rot, kv->head_dim, es) : 1;
     S2S_PAGED_DISPATCH(append_launch, (hipStream_t)stream, p, vec);
     S2S_LAUNCH_CHECK();
     return S2S_OK;
