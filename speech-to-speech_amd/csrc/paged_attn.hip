@@ -82,9 +82,10 @@ struct Span {
     int lo_all, hi_all;           // positions every row sees
 };
 __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, int nvr, Span& s) {
+    const int len = p.kv_len[b];
     session_rows(p.r, b, s.row0, s.n);
     if (s.n <= 0 || s.row0 >= p.r.T || vr0 >= s.n * p.G) return false;
-    s.len = max(0, min(p.kv_len[b], p.max_kv));
+    s.len = max(0, min(len, p.max_kv));
     s.past = s.len - s.n;
     const int t0 = vr0 / p.G, t1 = min(vr0 + nvr, s.n * p.G) - 1;
     const int t_last = t1 / p.G;
@@ -385,20 +386,23 @@ __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2]
 }
 
 // ---- few rows per session: every wave streams its own tiles from memory into registers -----------------------------------------------------
-// grid (q_tiles * n_splits, Hkv, B), 4 waves; wave w takes the split's tiles w, w + 4, ...; the four partial softmaxes meet in LDS at the end.  Bound
+// grid (q_tiles * n_splits, Hkv, B), W waves; wave w takes the split's tiles w, w + W, ...; their partial softmaxes meet in LDS at the end.  Bound
 // by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
 // the next values behind this tile's products, so both are in flight while the other is used.
 template <int KIND, int D>
 __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND>::frag_t frag_t;
-    constexpr int U = tile_u(KIND, D), TK = 32 * U, NS = D / 32, ND = D / 16;
-    __shared__ float so[2][16][D + 4];
-    __shared__ float sm[4][16], sl[4][16];
-    __shared__ alignas(16) unsigned char meta[KIND == KV_INT4 ? 4 * 2 * CodeMeta<D>::BYTES : 16];
+    constexpr int W = 4, U = tile_u(KIND, D), TK = 32 * U, NS = D / 32, ND = D / 16;
+    __shared__ float so[W / 2][16][D + 4];
+    __shared__ float sm[W][16], sl[W][16];
+    __shared__ alignas(16) unsigned char meta[KIND == KV_INT4 ? W * 2 * CodeMeta<D>::BYTES : 16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     unsigned char* own = meta + (KIND == KV_INT4 ? wave * 2 * CodeMeta<D>::BYTES : 0);
     const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
+    // Without a window the wave's first tile is known before the session's lengths are: its page number is asked for beside them.
+    const int first = split * p.chunk + wave * TK;
+    const int page0 = p.window > 0 ? -1 : page_raw(p.r, b, first);
     Span sp;
     if (!tile_span(p, b, vr0, 16, sp)) return;
     const int vr = vr0 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
@@ -424,16 +428,16 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
         const int ps_mask = (1 << p.r.ps_log2) - 1;
         const unsigned k_off = KeyTile<KIND, D>::lane_off(lane, l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
         const unsigned m_off = ValTile<KIND, D>::meta_off(lane, p.r.ps_log2);
-        int page = page_raw(p.r, b, kb), next = kb + 4 * TK < k1 ? page_raw(p.r, b, kb + 4 * TK) : -1;
+        int page = p.window > 0 ? page_raw(p.r, b, kb) : page0, next = kb + W * TK < k1 ? page_raw(p.r, b, kb + W * TK) : -1;
         {
             const long head = (long)(page_ok(p.r, page) ? page : 0) * p.r.Hkv + hk;
             kt.load(p, head, kb & ps_mask, k_off, lane);
             vt.load(p, head, kb & ps_mask, v_off, m_off);
         }
-        for (; kb < k1; kb += 4 * TK) {
-            const int nb = kb + 4 * TK;
+        for (; kb < k1; kb += W * TK) {
+            const int nb = kb + W * TK;
             const long nhead = (long)(page_ok(p.r, next) ? next : 0) * p.r.Hkv + hk;
-            const int after = nb + 4 * TK < k1 ? page_raw(p.r, b, nb + 4 * TK) : -1;
+            const int after = nb + W * TK < k1 ? page_raw(p.r, b, nb + W * TK) : -1;
             const int nat = nb < k1 ? nb & ps_mask : 0;
             f32x4_t s[U][2];
             kt.ready(own, lane);
@@ -467,21 +471,23 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    // four partial softmaxes of the same 16 columns -> one: common maximum first, then waves 2, 3 onto 0, 1, then 1 onto 0
+    // W partial softmaxes of the same 16 columns -> one: common maximum first, then the upper half of the waves onto the lower, and again
     if (g == 0) {
         sm[wave][l15] = m;
         sl[wave][l15] = l;
     }
     __syncthreads();
-    float M = fmaxf(fmaxf(sm[0][l15], sm[1][l15]), fmaxf(sm[2][l15], sm[3][l15]));
+    float M = sm[0][l15];
+#pragma unroll
+    for (int w = 1; w < W; ++w) M = fmaxf(M, sm[w][l15]);
     float L = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) L += sl[w][l15] * __builtin_amdgcn_exp2f(sm[w][l15] - M);
+    for (int w = 0; w < W; ++w) L += sl[w][l15] * __builtin_amdgcn_exp2f(sm[w][l15] - M);
     const float mine = __builtin_amdgcn_exp2f(m - M);
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] *= mine;
 #pragma unroll
-    for (int half = 2; half >= 1; half >>= 1) {
+    for (int half = W / 2; half >= 1; half >>= 1) {
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4_t*>(&so[wave - half][l15][d * 16 + g * 4]) = acc[d];
@@ -854,15 +860,20 @@ struct PagedPlan {
     bool tile;                    // attn_paged_tile_kernel
 };
 constexpr int tile_nc(int D) { return D == 256 ? 1 : 2; }           // 256 channels: what the registers hold
-// Which kernel, how many query tiles and splits: enough workgroups for two on every CU, no split shorter than 256 positions (a tile per wave).
+// Which kernel, how many query tiles and splits: enough workgroups to fill the CUs, no split shorter than 256 positions (a tile or two for every wave).
 static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, int max_kv, int causal, int window) {
     PagedPlan pl;
     const int G = H / kv->kv_heads;
-    pl.tile = (long)max_new * G > 32;
+    // The step kernel reads the pages again for every 16 rows; the tile kernel reads them once for 128 but leaves waves without rows idle and needs a barrier per
+    // tile.  Above 64 rows the second wins everywhere, up to 16 the first; in between it goes by how many (session, KV head) pairs there are to hide
+    // latencies behind.  us, step / tile: 24 rows, 128 pairs, 1500 positions, 128 channels: bf16 39 / 25, 4 bits 23 / 26, f32 69 / 85; 32 rows, 512
+    // pairs: bf16 116 / 73, 4 bits 52 / 47; 40 rows, 4 pairs, 4000 positions of 64 channels: bf16 9.8 / 11.1, 4 bits 9.0 / 12.5, f32 15 / 26.
+    const long rows_max = (long)max_new * G, pairs = (long)B * kv->kv_heads;
+    pl.tile = rows_max > 64 || (rows_max > 16 && pairs >= (paged_kind(kv) == KV_BF16 ? 64 : 256));
     const int rows = pl.tile ? 4 * 16 * tile_nc(kv->head_dim) : 16;
-    pl.q_tiles = cdiv((long)max_new * G, rows);
+    pl.q_tiles = cdiv(rows_max, rows);
     const long span = causal && window > 0 ? std::min<long>(max_kv, (long)window + cdiv(rows - 1, G) + 1 + 63) + 63 : max_kv;      // from a multiple of 64
-    const long groups = (long)B * kv->kv_heads * pl.q_tiles;
+    const long groups = pairs * pl.q_tiles;
     const long want = std::max<long>(1, (pl.tile ? 512 : 1024) / std::max<long>(1, groups));
     pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
     pl.n_splits = std::max(1, cdiv(span, pl.chunk));
@@ -871,8 +882,11 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
 }
 
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
-    if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
-    else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
+    if (p.tile) {
+        attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
+    } else {
+        attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
+    }
     if (p.n_splits > 8) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
     else if (p.n_splits > 1) attn_paged_join_kernel<T, D, 1><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }

@@ -177,6 +177,7 @@ class PagedKVCache:
         self.n_pages, self.kv_heads, self.page_size, self.head_dim, self.device = n, h, ps, d, k.device
         self._kv = native.PagedKVStruct(native.ptr(k), native.ptr(v), native.ptr(k_meta), native.ptr(v_meta), n, ps, h, d, KINDS[self.kind], native.dtype_code(self.dtype))
         self._ref = C.byref(self._kv)
+        self._ws: dict = {}  # workspace bytes by the sizes of a call
 
     def _sessions(self, table, lens, cu, rows, max_new, what):
         """-> (sessions, pages per session, bound of the new rows)."""
@@ -257,9 +258,13 @@ class PagedKVCache:
         lib, c = native.load(), 1 if causal else 0
         with _on_device(device) as stream:
             if workspace is None:
-                need = lib.s2s_op_attn_paged_ws(self._ref, H, b, T, max_new, max_kv, c, window)
-                if need < 0:
-                    native.check(int(need), "s2s_op_attn_paged_ws")
+                sizes = (H, b, T, max_new, max_kv, c, window)
+                need = self._ws.get(sizes)
+                if need is None:
+                    need = self.workspace_bytes(H, b, T, max_new=max_new, max_kv=max_kv, causal=causal, window=window)
+                    if len(self._ws) >= 4096:
+                        self._ws.clear()
+                    self._ws[sizes] = need
                 if need:
                     workspace = torch.empty(need, dtype=torch.uint8, device=device)
             elif workspace.device != device or not workspace.is_contiguous():
