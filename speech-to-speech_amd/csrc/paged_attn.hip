@@ -322,6 +322,9 @@ __device__ __forceinline__ void probs(const float (&x)[8], bf16x8_t& hi) {
 // The running maximum is raised only when a score exceeds it by more than 8 (in log2): P stays below 2^8, sums and products are f32, so nothing is lost,
 // and the usual step needs no cross-lane maximum and no rescaling.
 constexpr float MAX_SLACK = 8.f;
+// The maximum that is kept lies this far below the true one, so that the weights fill the upper range of float16 (up to 2^15) and a long tail of small ones does
+// not fall off its lower end: 2^-32 of the largest weight is still seen.  bf16 and f32 have room on both sides.
+constexpr float max_bias(int kind) { return kind == KV_INT4 ? 7.f : 0.f; }
 constexpr float NO_MAX = -3e38f;                  // finite, so that masked scores (-inf) minus it stay -inf
 
 __device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -344,13 +347,13 @@ __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2]
             x[u][e] = fmaf(s[u][e >> 2][e & 3], sc, -m);
             mx = fmaxf(mx, x[u][e]);
         }
-    if (__any(mx > MAX_SLACK)) {
-        float mn = m;
+    if (__any(mx > MAX_SLACK + max_bias(KIND))) {
+        float mn = m + max_bias(KIND);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[u][e >> 2][e & 3] * sc);
-        mn = max_over_groups(mn);
+        mn = max_over_groups(mn) - max_bias(KIND);
         const float a = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= a;
@@ -656,17 +659,17 @@ __device__ __forceinline__ void tile_step(const unsigned char* buf, const LdsOff
                 x[c][u][e] = fmaf(s[c][u][e >> 2][e & 3], sc[c], -m[c]);
                 mx = fmaxf(mx, x[c][u][e]);
             }
-        raise |= mx > MAX_SLACK;
+        raise |= mx > MAX_SLACK + max_bias(KIND);
     }
     if (__any(raise)) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            float mn = m[c];
+            float mn = m[c] + max_bias(KIND);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) mn = fmaxf(mn, s[c][u][e >> 2][e & 3] * sc[c]);
-            mn = max_over_groups(mn);
+            mn = max_over_groups(mn) - max_bias(KIND);
             const float a = __builtin_amdgcn_exp2f(m[c] - mn);
             m[c] = mn;
             l[c] *= a;
@@ -922,6 +925,8 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(q && o && kv_len_dev, "attn_paged: null buffer");
     const PagedPlan pl = paged_plan(kv, H, B, p.r.max_new, max_kv, causal, window);
+    S2S_REQUIRE((int64_t)pl.q_tiles * pl.n_splits * kv->kv_heads * B < (1LL << 31) && (int64_t)T * H < (1LL << 31),
+                "attn_paged: %d sessions of up to %d rows are too many for one call", B, max_new);
     const int64_t need = pl.n_splits == 1 ? 0 : (int64_t)pl.n_splits * T * H * (kv->head_dim + 1) * 4;
     S2S_REQUIRE(need == 0 || (ws_dev && ws_bytes >= need && !((uintptr_t)ws_dev & 15)), "attn_paged: workspace of %lld bytes, 16-byte aligned, needed (got %lld)",
                 (long long)need, (long long)ws_bytes);

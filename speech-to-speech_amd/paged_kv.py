@@ -190,7 +190,7 @@ class PagedKVCache:
                 raise ValueError(f"without cu there is one row per session ({rows} rows, {b} sessions, max_new {max_new})")
             return b, cols, 1
         _ints(cu, b + 1, self.device, "cu")
-        return b, cols, max(1, rows if max_new is None else max_new)
+        return b, cols, max(1, rows if max_new is None else min(max_new, rows))
 
     def append(self, k, v, table, start, cu=None, *, max_new=None, cos=None, sin=None, interleaved: bool = False, q=None, q_out=None):
         """Store every session's new rows behind the ``start`` positions its pages hold, keys turned to their positions (``cos`` / ``sin`` None: as they come).
@@ -250,6 +250,9 @@ class PagedKVCache:
         b, cols, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
         if max_kv is None:
             max_kv = cols * self.page_size
+        elif not 0 <= max_kv <= cols * self.page_size:
+            raise ValueError(f"max_kv: 0 .. {cols * self.page_size} in {cols} pages of {self.page_size}, got {max_kv}")
+        window = min(window, 1 << 30)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=device)
         To, _, o_rs = _rows(out, H, dim, self.dtype, device, "out")

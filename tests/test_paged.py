@@ -50,6 +50,9 @@ def test_bad_calls_are_refused():
         assert attend(kv, cols=1024, max_kv=65536, ws=ws, ws_bytes=n) == -1
         assert b"workspace" in lib.s2s_last_error()
     assert lib.s2s_op_attn_paged_ws(C.byref(kv), 4, 0, 0, 1, 512, 1, 0) == 0
+    # more workgroups than a launch takes, more (row, head) pairs than an index holds
+    assert attend(handle(kv_heads=1024), H=1024, cu=P, B=60000, T=2**26, max_new=2**26) == -1 and b"too many" in lib.s2s_last_error()
+    assert attend(handle(kv_heads=1024), H=4096, cu=P, B=1, T=2**20, max_new=1) == -1 and b"too many" in lib.s2s_last_error()
     for kw in (dict(rot=0), dict(rot=129), dict(rot=130), dict(max_pos=0), dict(sin=0), dict(q=P), dict(q=P, q_out=P), dict(q=P, q_out=P, H=4, cos=0, sin=0), dict(k=0), dict(start=0),
                dict(table=0), dict(T=3), dict(max_new=4)):
         assert append(kv, **kw) == -1, kw
@@ -75,7 +78,7 @@ def test_python_entry_points_refuse_what_does_not_fit():
            lambda: c.append(rows(), rows(), table, i(0, 0), cos=cos), lambda: c.append(rows(), rows(), table, i(0, 0), cos=cos.double(), sin=sin.double()),
            lambda: c.append(torch.zeros(2, 64, 2, dtype=torch.bfloat16).transpose(1, 2), rows(), table, i(0, 0)),
            lambda: c.append(rows(), rows(), table, i(0, 0), cos=cos, sin=sin, q=rows(4), q_out=rows(3)), lambda: c.attend(rows(4, 2, 32), table, i(1, 1)),
-           lambda: c.attend(rows(4), table, i(1, 1), out=rows(4, 3)), lambda: c.attend(rows(4), table, i(1, 1), max_new=2), lambda: c.read(table, i(0, 0), i(0, 1, 2)),
+           lambda: c.attend(rows(4), table, i(1, 1), out=rows(4, 3)), lambda: c.attend(rows(4), table, i(1, 1), max_new=2), lambda: c.attend(rows(4), table, i(1, 1), max_kv=129), lambda: c.attend(rows(4), table, i(1, 1), max_kv=2**32), lambda: c.read(table, i(0, 0), i(0, 1, 2)),
            lambda: rope(rows(), i(0), cos, sin), lambda: rope(rows(), i(0, 1), cos, sin[:4]), lambda: rope(rows(), i(0, 1), cos, sin, out=rows(3)),
            lambda: PagedKVCache(4, 2, 64, kind="int3", device="cpu"), lambda: PagedKVCache(4, 2, 64, kind="int4", dtype=torch.float32, device="cpu"),
            lambda: PagedKVCache.adopt(c.k, c.k[:3]), lambda: PagedKVCache.adopt(c.k, c.v, c.k), lambda: rope_tables(7, 4, device="cpu"), lambda: rope_tables(8, 4, scaling="odd", device="cpu"),

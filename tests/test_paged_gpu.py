@@ -356,6 +356,29 @@ def test_attend_with_scores_far_apart_and_infinite():
     assert (o[0, 0].double() - p @ v[keep, 0].double()).abs().max() < 1e-5
 
 
+def test_attend_keeps_a_long_tail_of_small_weights():
+    """One position with nearly all the weight and 60000 of 2^-29 to 2^-25 of it whose values point the same way: together 1e-4 to 2e-3 of the result, which float16 weights
+    below 2^-24 of the largest would drop."""
+    Hkv, D, ps, n = 1, 64, 64, 60000
+    table, n_pages = make_table([n], ps, 0, 1)
+    for kind, dtype in KINDS:
+        for tail in (-29, -27, -25):
+            cache = poisoned(n_pages, Hkv, D, ps, kind, dtype)
+            k, v = torch.zeros(n, Hkv, D), torch.ones(n, Hkv, D)
+            k[0, 0, :32], v[0] = 1.0, 0.0
+            cache.append(k.to(dtype).to(DEV), v.to(dtype).to(DEV), table.to(DEV), i32([0]), i32([0, n]), max_new=n)
+            for rows in (1, 70):
+                q = torch.full((rows, 1, D), 1.0, dtype=dtype, device=DEV)
+                scale = -tail / 32 * 0.6931471805599453
+                o = cache.attend(q, table.to(DEV), i32([n]), i32([0, rows]), max_new=rows, causal=False, scale=scale).cpu().double()
+                w = (n - 1) * 2.0**tail
+                want = w / (1 + w)
+                # the score of position 0 is exact up to its f32 product (2^-22 of |tail|), a weight is off by half a step of its type (2^-8 at most), and of float16 by
+                # 2^-25 of 2^-7 of the largest at most; the sums of n weights in f32 by n half steps at worst
+                tol = want * (2.0**-8 + abs(tail) * 2.0**-21 + n * 2.0**-24) + (n * 2.0**-32 if kind == "int4" else 0) + want * torch.finfo(dtype).eps / 2
+                assert (o - want).abs().max() <= tol, (kind, dtype, tail, rows, float((o - want).abs().max() / want))
+
+
 def test_offsets_behind_32_bits():
     """Pages whose elements (and bytes) lie behind 2^32, and a row buffer just as long."""
     for kind, dtype, n_pages in (("model", BF, 34000), ("int4", BF, 70000)):
