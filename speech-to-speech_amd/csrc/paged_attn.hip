@@ -403,9 +403,6 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
     unsigned char* own = meta + (KIND == KV_INT4 ? wave * 2 * CodeMeta<D>::BYTES : 0);
     const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
-    // Without a window the wave's first tile is known before the session's lengths are: its page number is asked for beside them.
-    const int first = split * p.chunk + wave * TK;
-    const int page0 = p.window > 0 ? -1 : page_raw(p.r, b, first);
     Span sp;
     if (!tile_span(p, b, vr0, 16, sp)) return;
     const int vr = vr0 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
@@ -431,7 +428,7 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
         const int ps_mask = (1 << p.r.ps_log2) - 1;
         const unsigned k_off = KeyTile<KIND, D>::lane_off(lane, l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
         const unsigned m_off = ValTile<KIND, D>::meta_off(lane, p.r.ps_log2);
-        int page = p.window > 0 ? page_raw(p.r, b, kb) : page0, next = kb + W * TK < k1 ? page_raw(p.r, b, kb + W * TK) : -1;
+        int page = page_raw(p.r, b, kb), next = kb + W * TK < k1 ? page_raw(p.r, b, kb + W * TK) : -1;
         {
             const long head = (long)(page_ok(p.r, page) ? page : 0) * p.r.Hkv + hk;
             kt.load(p, head, kb & ps_mask, k_off, lane);
@@ -863,7 +860,7 @@ struct PagedPlan {
     bool tile;                    // attn_paged_tile_kernel
 };
 constexpr int tile_nc(int D) { return D == 256 ? 1 : 2; }           // 256 channels: what the registers hold
-// Which kernel, how many query tiles and splits: enough workgroups to fill the CUs, no split shorter than 256 positions (a tile or two for every wave).
+// Which kernel, how many query tiles and splits: enough workgroups to fill the CUs.
 static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, int max_kv, int causal, int window) {
     PagedPlan pl;
     const int G = H / kv->kv_heads;
@@ -878,7 +875,9 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
     const long span = causal && window > 0 ? std::min<long>(max_kv, (long)window + cdiv(rows - 1, G) + 1 + 63) + 63 : max_kv;      // from a multiple of 64
     const long groups = pairs * pl.q_tiles;
     const long want = std::max<long>(1, (pl.tile ? 512 : 1024) / std::max<long>(1, groups));
-    pl.chunk = std::max(256, cdiv(cdiv(span, want), 256) * 256);
+    // a split is a tile for every wave at least; where one split of 256 positions does, the second launch costs more than it saves
+    const int least = pl.tile ? 256 : 4 * 32 * tile_u(paged_kind(kv), kv->head_dim);
+    pl.chunk = span <= 256 ? 256 : std::max(least, cdiv(cdiv(span, want), least) * least);
     pl.n_splits = std::max(1, cdiv(span, pl.chunk));
     if (pl.n_splits == 1) pl.chunk = 1 << 30;
     return pl;
