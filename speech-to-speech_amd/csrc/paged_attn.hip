@@ -700,6 +700,20 @@ __device__ __forceinline__ void tile_step(const unsigned char* buf, const LdsOff
         }
 }
 
+// The session whose kv_len is the i-th largest (up to 64 sessions, a lane each: beyond that there are workgroups enough for the order not to matter).  Long
+// sessions are begun first, so that what is left at the end is short (ragged prompts: 462 -> 437 us; 16 sessions over 4-bit pages, all workgroups resident at once, so
+// that long ones share a CU with short ones: 142 -> 124 us).
+__device__ __forceinline__ int session_by_length(const PagedAttn& p, int i, int lane) {
+    if (p.r.B > 64) return i;
+    const int len = lane < p.r.B ? p.kv_len[lane] : -1;
+    int rank = 0;
+    for (int j = 0; j < p.r.B; ++j) {
+        const int other = __builtin_amdgcn_readlane(len, j);
+        rank += other > len || (other == len && j < lane) ? 1 : 0;
+    }
+    return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(lane < p.r.B && rank == i)) - 1);
+}
+
 template <int KIND, int D, int NC>
 __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_paged_tile_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
@@ -720,7 +734,7 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
         pair = blockIdx.x / per;
         w = blockIdx.x % per;
     }
-    const int b = pair / p.r.Hkv, hk = pair % p.r.Hkv, split = w % p.n_splits, vr0 = (p.q_tiles - 1 - w / p.n_splits) * 4 * RW;
+    const int b = session_by_length(p, pair / p.r.Hkv, lane), hk = pair % p.r.Hkv, split = w % p.n_splits, vr0 = (p.q_tiles - 1 - w / p.n_splits) * 4 * RW;
     Span sp, sw;
     if (!tile_span(p, b, vr0, 4 * RW, sp)) return;
     if (!tile_span(p, b, vr0 + wave * RW, RW, sw)) sw.lo = sw.hi = sw.lo_all = sw.hi_all = 0;      // no rows: help with the tiles only
