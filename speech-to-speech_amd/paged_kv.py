@@ -39,23 +39,18 @@ def _require(cond, msg: str) -> None:
 # The checks of a call's tensors cost as much as its launch: they are plain comparisons, and a message is put together only to be raised.
 
 
-class _on_device:
-    """Make the tensors' device current for the call (nothing where it is) and give torch's current stream there."""
-
-    def __init__(self, device):
-        if device.type != "cuda":
-            raise ValueError(f"tensors on {device}: the operators run on a GPU only")
-        self.index = device.index
-        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard:
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard:
-            self.guard.__exit__(*exc)
+def _call(device, name, fn, *args):
+    """fn(torch's current stream on ``device``, *args) with that device current (it is: the usual case, where torch's guard would cost as much as the launch)."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors on {device}: the operators run on a GPU only")
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    if status:
+        native.check(status, name)
 
 
 def _ints(t, n, device, what):
@@ -132,9 +127,8 @@ def rope(x, positions, cos, sin, *, interleaved: bool = False, out=None):
     elif out.shape != shape or out.dtype is not x.dtype or out.device != device or (out.stride(2) != 1 and out.numel()):
         raise ValueError(f"out must match x, got {out.dtype} {tuple(out.shape)} on {out.device}")
     xs, os = x.stride(), out.stride()
-    with _on_device(device) as stream:
-        native.check(native.load().s2s_op_rope(stream, x.data_ptr(), xs[0], xs[1], out.data_ptr(), os[0], os[1], positions.data_ptr(), cp, sp, n, shape[0], shape[1], shape[2], rot,
-                                               1 if interleaved else 0, native.dtype_code(x.dtype)), "s2s_op_rope")
+    _call(device, "s2s_op_rope", native.load().s2s_op_rope, x.data_ptr(), xs[0], xs[1], out.data_ptr(), os[0], os[1], positions.data_ptr(), cp, sp, n, shape[0], shape[1], shape[2],
+          rot, 1 if interleaved else 0, native.dtype_code(x.dtype))
     return out
 
 
@@ -206,17 +200,16 @@ class PagedKVCache:
                 raise ValueError("queries are turned: cos / sin needed")
             Tq, H, q_rs = _rows(q, None, dim, dtype, device, "q")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=dtype, device=device)
-            To, _, qo_rs = _rows(q_out, H, dim, dtype, device, "q_out")
-            if To != Tq:
-                raise ValueError(f"q_out: {Tq} rows needed, got {To}")
+                q_out, qo_rs = torch.empty((Tq, H, dim), dtype=dtype, device=device), H * dim
+            else:
+                To, _, qo_rs = _rows(q_out, H, dim, dtype, device, "q_out")
+                if To != Tq:
+                    raise ValueError(f"q_out: {Tq} rows needed, got {To}")
             qp, qop = q.data_ptr(), q_out.data_ptr()
         if Tv != T or Tq != T:
             raise ValueError(f"k, v and q need the same rows, got {T}, {Tv} and {Tq}")
-        with _on_device(device) as stream:
-            native.check(native.load().s2s_op_kv_append_paged(stream, self._ref, k.data_ptr(), k_rs, v.data_ptr(), v_rs, qp, q_rs, qop, qo_rs, H, table.data_ptr(), cols,
-                                                              start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, T, max_new, cp, sp, n, rot, 1 if interleaved else 0),
-                         "s2s_op_kv_append_paged")
+        _call(device, "s2s_op_kv_append_paged", native.load().s2s_op_kv_append_paged, self._ref, k.data_ptr(), k_rs, v.data_ptr(), v_rs, qp, q_rs, qop, qo_rs, H, table.data_ptr(), cols,
+              start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, T, max_new, cp, sp, n, rot, 1 if interleaved else 0)
         return q_out if H else None
 
     def read(self, table, start, cu=None, rows=None, *, max_new=None):
@@ -228,9 +221,8 @@ class PagedKVCache:
         b, cols, max_new = self._sessions(table, start, cu, rows, max_new, "start")
         shape = (rows, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
-        with _on_device(self.device) as stream:
-            native.check(native.load().s2s_op_kv_read_paged(stream, self._ref, table.data_ptr(), cols, start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, rows, max_new,
-                                                            k.data_ptr(), v.data_ptr(), self.kv_heads * self.head_dim), "s2s_op_kv_read_paged")
+        _call(self.device, "s2s_op_kv_read_paged", native.load().s2s_op_kv_read_paged, self._ref, table.data_ptr(), cols, start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, rows,
+              max_new, k.data_ptr(), v.data_ptr(), self.kv_heads * self.head_dim)
         return k, v
 
     def workspace_bytes(self, heads: int, sessions: int, rows: int, *, max_new: int = 1, max_kv: int, causal: bool = True, window: int = 0) -> int:
@@ -254,26 +246,25 @@ class PagedKVCache:
             raise ValueError(f"max_kv: 0 .. {cols * self.page_size} in {cols} pages of {self.page_size}, got {max_kv}")
         window = min(window, 1 << 30)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        To, _, o_rs = _rows(out, H, dim, self.dtype, device, "out")
-        if To != T:
-            raise ValueError(f"out: {T} rows needed, got {To}")
-        lib, c = native.load(), 1 if causal else 0
-        with _on_device(device) as stream:
-            if workspace is None:
-                sizes = (H, b, T, max_new, max_kv, c, window)
-                need = self._ws.get(sizes)
-                if need is None:
-                    need = self.workspace_bytes(H, b, T, max_new=max_new, max_kv=max_kv, causal=causal, window=window)
-                    if len(self._ws) >= 4096:
-                        self._ws.clear()
-                    self._ws[sizes] = need
-                if need:
-                    workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            elif workspace.device != device or not workspace.is_contiguous():
-                raise ValueError(f"workspace: contiguous on {device} needed")
-            ws, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-            native.check(lib.s2s_op_attn_paged(stream, self._ref, q.data_ptr(), q_rs, out.data_ptr(), o_rs, H, table.data_ptr(), cols, kv_len.data_ptr(),
-                                               0 if cu is None else cu.data_ptr(), b, T, max_new, max_kv, dim ** -0.5 if scale is None else scale, c, window, ws, ws_bytes),
-                         "s2s_op_attn_paged")
+            out, o_rs = torch.empty((T, H, dim), dtype=self.dtype, device=device), H * dim
+        else:
+            To, _, o_rs = _rows(out, H, dim, self.dtype, device, "out")
+            if To != T:
+                raise ValueError(f"out: {T} rows needed, got {To}")
+        c = 1 if causal else 0
+        if workspace is None:
+            sizes = (H, b, T, max_new, max_kv, c, window)
+            need = self._ws.get(sizes)
+            if need is None:
+                need = self.workspace_bytes(H, b, T, max_new=max_new, max_kv=max_kv, causal=causal, window=window)
+                if len(self._ws) >= 4096:
+                    self._ws.clear()
+                self._ws[sizes] = need
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace: contiguous on {device} needed")
+        ws, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        _call(device, "s2s_op_attn_paged", native.load().s2s_op_attn_paged, self._ref, q.data_ptr(), q_rs, out.data_ptr(), o_rs, H, table.data_ptr(), cols, kv_len.data_ptr(),
+              0 if cu is None else cu.data_ptr(), b, T, max_new, max_kv, dim ** -0.5 if scale is None else scale, c, window, ws, ws_bytes)
         return out
