@@ -260,7 +260,7 @@ int32_t s2s_op_attention(void* stream, const void* q, int64_t q_rs, const void* 
  * stored, its positions are not attended to.  A page that is written must belong to one session only; pages that are only read may be shared.
  * cu_dev int32 [B + 1]: session b's new rows are cu[b] .. cu[b + 1] - 1 of the row buffers (T rows); NULL: one row per session (T = B).
  * max_new: host-side bound of every session's new rows; max_kv: of every kv_len.  Buffers are read with row strides *_rs in elements, the
- * heads of a row lie next to each other.  Rows at and behind cu[B] are left as they are. */
+ * heads of a row lie next to each other.  Rows at and behind cu[B] are left as they are; rows of a session beyond max_new are not computed. */
 #define S2S_KV_MODEL 0
 #define S2S_KV_INT4 1
 typedef struct s2s_paged_kv {

@@ -2,7 +2,7 @@
 //
 // One tile of TK positions, per wave, with the scores TRANSPOSED so that a lane keeps one query row (column) for good:
 //   S^T [16 positions][16 rows] = K Q^T       A = key rows from the page, B = query rows held in registers
-//   P^T = exp2(S^T * scale * log2 e - m)      running maximum m and sum l per column: two shuffles per tile, nothing through LDS
+//   P^T = exp2(S^T * scale * log2 e - m)      running maximum m and sum l per column, l per lane until the end: nothing through LDS
 //   O^T [16 channels][16 rows] += V^T P^T     A = value rows of the transposed page, B = P^T straight from the registers S^T was in
 // The C layout of a 16 x 16 product puts rows 4 g + r (g = lane / 16) into lane g's registers, the B layout wants 8 neighbours per lane: the key
 // row that score tile (u, t) reads at index m is chosen as position (m / 4) 8 U + 8 u + 4 t + m % 4, and lane g holds the positions 8 U g + 8 u .. + 7
@@ -180,7 +180,7 @@ template <typename V> __device__ __forceinline__ V ld_once(const void* base, uns
 template <int KIND, int D> struct KeyTile {       // bf16, f32: octets of the U x 2 rows this lane stands for
     static constexpr int U = tile_u(KIND, D), EB = KIND == KV_F32 ? 4 : 2;
     typename KvT<KIND>::frag_t f[U][2][D / 32];
-    static __device__ __forceinline__ unsigned lane_off(int, int l15, int g) { return (((l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8) * EB; }
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return (((l15 >> 2) * 8 * U + (l15 & 3)) * D + g * 8) * EB; }
     __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, int) {
         const char* base = (const char*)p.kc + ((head << p.r.ps_log2) + at) * D * EB;
 #pragma unroll
@@ -231,7 +231,7 @@ template <int D> struct KeyTile<KV_INT4, D> {
     typedef unsigned words_t __attribute__((ext_vector_type(NS)));
     words_t w[U][2];
     typename M::words_t m;
-    static __device__ __forceinline__ unsigned lane_off(int, int l15, int g) { return ((l15 >> 2) * 8 * U + (l15 & 3)) * (D / 2) + g * NS * 4; }
+    static __device__ __forceinline__ unsigned lane_off(int l15, int g) { return ((l15 >> 2) * 8 * U + (l15 & 3)) * (D / 2) + g * NS * 4; }
     __device__ __forceinline__ void load(const PagedAttn& p, long head, int at, unsigned off, int lane) {
         const long row = (head << p.r.ps_log2) + at;
         const char* base = (const char*)p.kc + row * (D / 2);
@@ -391,7 +391,8 @@ __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2]
 // ---- few rows per session: every wave streams its own tiles from memory into registers -----------------------------------------------------
 // grid (q_tiles * n_splits, Hkv, B), W waves; wave w takes the split's tiles w, w + W, ...; their partial softmaxes meet in LDS at the end.  Bound
 // by HBM: keys and values go straight into the operand registers, the loads of the next keys are issued before this tile's softmax and those of
-// the next values behind this tile's products, so both are in flight while the other is used.
+// the next values behind this tile's products, so both are in flight while the other is used.  512 sessions of up to 1531 positions, 16 / 8 heads of 128, bf16: 304 us,
+// 5.5 TB/s (a large copy reaches 4.9); 4 bits, 64 x 1500 positions of 20 heads of 64: 31.6 us, 4.9 TB/s; 7 sessions of up to 100021: 104 us, 5.0 TB/s.
 template <int KIND, int D>
 __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attn_paged_step_kernel(PagedAttn p) {
     typedef typename KvT<KIND>::row_t T;
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
         KeyTile<KIND, D> kt;
         ValTile<KIND, D> vt;
         const int ps_mask = (1 << p.r.ps_log2) - 1;
-        const unsigned k_off = KeyTile<KIND, D>::lane_off(lane, l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
+        const unsigned k_off = KeyTile<KIND, D>::lane_off(l15, g), v_off = ValTile<KIND, D>::lane_off(l15, g, p.r.ps_log2);
         const unsigned m_off = ValTile<KIND, D>::meta_off(lane, p.r.ps_log2);
         int page = page_raw(p.r, b, kb), next = kb + W * TK < k1 ? page_raw(p.r, b, kb + W * TK) : -1;
         {
@@ -517,9 +518,11 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
 
 // ---- many rows per session: a workgroup's tile of query rows shares every tile of positions through LDS ----------------------------------------
 // 4 waves x NC x 16 columns.  Tiles of keys and values go from the page into LDS without passing registers (4-bit codes: through registers, as
-// float16), a double buffer and one barrier per tile.  Octets are stored at index o ^ f(row): the 8 lanes that read together hold rows whose f differs,
-// so the 16-byte reads hit every bank once.  Per 32 positions a wave reads 2 KiB x D / 64 of keys and of values for 16 NC columns; at NC = 2 the LDS reads
-// take as long as the products.
+// float16), a double buffer and one barrier per tile.  Octets are stored at index o ^ f(row), f different for the 16 lanes that read together, so that
+// the 16-byte reads hit every bank once (SQ_LDS_BANK_CONFLICT 0; 53 M cycles with 8 values of f).  NC = 2: one operand read serves two products.
+// Bound, at 428 GFLOP of bf16 prompts (437 us, 980 TFLOP/s, the library's 8192^3 product reaches 1210): a tile step is the 1024 cycles of its products plus the
+// 800 of its softmax, which two waves per SIMD overlap only in part, at 2.0 - 2.1 GHz.  Scores of tile t + 1 beside the exponentials of tile t, in the
+// compiler's order or a prescribed one, 32-position tiles at 3 waves per SIMD and 48 rows per wave (spills) were not faster.
 template <int KIND, int D> struct LdsTile {
     static constexpr int U = tile_u(KIND, D), TK = 32 * U;
     static constexpr int EB = KIND == KV_F32 ? 4 : 2, OB = 8 * EB;  // bytes per element and per octet in LDS
@@ -773,8 +776,8 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
         dma.start(p, lds, page, hk, k0 & ps_mask, wave);
     }
     for (int kb = k0; kb < k1; kb += TK) {
-        __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed
-        __builtin_amdgcn_s_barrier();              // everyone's has, and everyone is done with the other buffer
+        __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed (loads to LDS count as loads, not as LDS writes)
+        __syncthreads();                           // everyone's has, and everyone is done with the other buffer
         unsigned char* buf = lds + cur * L::BYTES;
         unsigned char* other = lds + (cur ^ 1) * L::BYTES;
         const int after = kb + 2 * TK < k1 ? page_raw(p.r, b, kb + 2 * TK) : -1;
@@ -898,11 +901,8 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
 }
 
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
-    if (p.tile) {
-        attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
-    } else {
-        attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
-    }
+    if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
+    else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
     if (p.n_splits > 8) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
     else if (p.n_splits > 1) attn_paged_join_kernel<T, D, 1><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }
@@ -917,6 +917,10 @@ static int attn_paged_sizes(const s2s_paged_kv* kv, int H, int B, int T, int max
     S2S_REQUIRE(B >= 0 && B <= 65535 && T >= 0 && max_new >= 1, "attn_paged: B=%d T=%d max_new=%d", B, T, max_new);
     S2S_REQUIRE(max_kv >= 0 && max_kv <= 1 << 30, "attn_paged: max_kv=%d", max_kv);
     S2S_REQUIRE(window >= 0 && (window == 0 || causal), "attn_paged: a window (%d) needs the causal mask", window);
+    S2S_REQUIRE((int64_t)T * H < (1LL << 31), "attn_paged: %d rows of %d heads are too many for one call", T, H);
+    if (B == 0 || T == 0) return S2S_OK;
+    const PagedPlan pl = paged_plan(kv, H, B, std::min(max_new, T), max_kv, causal, window);
+    S2S_REQUIRE((int64_t)pl.q_tiles * pl.n_splits * kv->kv_heads * B < (1LL << 31), "attn_paged: %d sessions of up to %d rows are too many for one call", B, max_new);
     return S2S_OK;
 }
 
@@ -938,8 +942,6 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(q && o && kv_len_dev, "attn_paged: null buffer");
     const PagedPlan pl = paged_plan(kv, H, B, p.r.max_new, max_kv, causal, window);
-    S2S_REQUIRE((int64_t)pl.q_tiles * pl.n_splits * kv->kv_heads * B < (1LL << 31) && (int64_t)T * H < (1LL << 31),
-                "attn_paged: %d sessions of up to %d rows are too many for one call", B, max_new);
     const int64_t need = pl.n_splits == 1 ? 0 : (int64_t)pl.n_splits * T * H * (kv->head_dim + 1) * 4;
     S2S_REQUIRE(need == 0 || (ws_dev && ws_bytes >= need && !((uintptr_t)ws_dev & 15)), "attn_paged: workspace of %lld bytes, 16-byte aligned, needed (got %lld)",
                 (long long)need, (long long)ws_bytes);
