@@ -318,6 +318,25 @@ def test_attend_prompts(kind, dtype, new, kv, Hkv, H, D, ps):
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+def test_attend_many_sessions_with_prompts(kind, dtype):
+    """More sessions than are sorted by length (64), exactly as many, and pair counts that are and are not a multiple of 8."""
+    r = random.Random(5)
+    for B, Hkv in ((70, 2), (64, 1), (65, 1), (13, 8)):
+        kv = [r.choice([0, 1, 40, 64, 100, 333]) for _ in range(B)]
+        new = [r.choice([0, 1, 2, 33, 70]) for _ in range(B)]
+        check_attention(new, kv, Hkv, 2 * Hkv, 64, 64, kind, dtype, seed=B, few=False)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("rows", [17, 24, 32, 33, 64, 65])
+def test_attend_row_counts_around_the_kernels_borders(kind, dtype, rows):
+    """(row, head) pairs per KV head at which one kernel hands over to the other, with few and with many sessions."""
+    check_attention([rows, 1], [200, 77], 1, 1, 64, 64, kind, dtype, seed=rows, few=False)
+    check_attention([1] * 5, [70, 1, 300, 64, 2], 1, rows, 128, 64, kind, dtype, seed=rows, few=False)
+    check_attention([rows // 8] * 40, [rows // 8 + 7 * (i % 9) for i in range(40)], 8, 64, 64, 64, kind, dtype, seed=rows, few=False)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 def test_attend_skips_positions_without_a_page(kind, dtype):
     check_attention([1, 1], [500, 300], 2, 4, 128, 64, kind, dtype, holes=[(0, 0), (0, 3), (1, 4)])
     check_attention([1], [64], 2, 4, 64, 64, kind, dtype, holes=[(0, 0)])      # nothing left: zero
@@ -477,6 +496,48 @@ def test_captured_step_replays_with_other_lengths(kind, dtype):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
         start += 1
         kv += 1
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_queries_in_place_and_a_captured_prompt(kind, dtype):
+    """Appending with queries turned in place gives the rows of the call with a buffer for them; the prompt in a graph gives the eager result, replay after replay."""
+    Hkv, H, D, ps = 2, 4, 128, 64
+    cos, sin = rope_tables(64, 512, device=DEV)
+    for new, past in (([1, 1, 1], [5, 64, 200]), ([90, 3, 41], [0, 64, 100])):
+        T, cu, total = sum(new), i32(ragged(new)), [a + b for a, b in zip(new, past)]
+        table, n_pages = make_table(total, ps, 0, T)
+        tb, start, kv = table.to(DEV), i32(past), i32(total)
+        cache = poisoned(n_pages, Hkv, D, ps, kind, dtype)
+        kp, vp = randn(sum(past), Hkv, D, seed=1, dtype=dtype).to(DEV), randn(sum(past), Hkv, D, seed=2, dtype=dtype).to(DEV)
+        cache.append(kp, vp, tb, i32([0] * 3), i32(ragged(past)), max_new=max(past))
+        q, k, v = (torch.zeros(T, h, D, dtype=dtype, device=DEV) for h in (H, Hkv, Hkv))
+        args = dict(max_new=max(new), cos=cos, sin=sin)
+        out = torch.empty_like(q)
+
+        def turn():
+            w = cache.append(k, v, tb, start, cu, q=q, **args)
+            cache.attend(w, tb, kv, cu, max_new=max(new), max_kv=max(total), out=out)
+            return w
+
+        turn()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            turned = turn()
+        for i in range(3):
+            for t, s in ((q, 10), (k, 20), (v, 30)):
+                t.copy_(randn(*t.shape, seed=s + i, dtype=dtype))
+            graph.replay()
+            torch.cuda.synchronize()
+            replayed, was = out.clone(), turned.clone()
+            out.zero_()
+            again = turn()
+            torch.cuda.synchronize()
+            assert torch.equal(again, was) and torch.equal(out, replayed)
+            inplace = q.clone()
+            assert cache.append(k, v, tb, start, cu, q=inplace, q_out=inplace, **args) is inplace
+            assert torch.equal(inplace, was)
 
 
 def test_other_streams_and_repeated_calls_agree():
