@@ -123,7 +123,7 @@ def rope(x, positions, cos, sin, *, interleaved: bool = False, out=None):
     _ints(positions, shape[0], device, "positions")
     n, rot, cp, sp = _tables(cos, sin, device)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not x.dtype or out.device != device or (out.stride(2) != 1 and out.numel()):
         raise ValueError(f"out must match x, got {out.dtype} {tuple(out.shape)} on {out.device}")
     xs, os = x.stride(), out.stride()
@@ -200,7 +200,7 @@ class PagedKVCache:
                 raise ValueError("queries are turned: cos / sin needed")
             Tq, H, q_rs = _rows(q, None, dim, dtype, device, "q")
             if q_out is None:
-                q_out, qo_rs = torch.empty((Tq, H, dim), dtype=dtype, device=device), H * dim
+                q_out, qo_rs = torch.empty_like(q, memory_format=torch.contiguous_format), H * dim
             else:
                 To, _, qo_rs = _rows(q_out, H, dim, dtype, device, "q_out")
                 if To != Tq:
@@ -246,7 +246,7 @@ class PagedKVCache:
             raise ValueError(f"max_kv: 0 .. {cols * self.page_size} in {cols} pages of {self.page_size}, got {max_kv}")
         window = min(window, 1 << 30)
         if out is None:
-            out, o_rs = torch.empty((T, H, dim), dtype=self.dtype, device=device), H * dim
+            out, o_rs = torch.empty_like(q, memory_format=torch.contiguous_format), H * dim
         else:
             To, _, o_rs = _rows(out, H, dim, self.dtype, device, "out")
             if To != T:
