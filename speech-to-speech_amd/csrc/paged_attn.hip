@@ -25,11 +25,13 @@ struct PagedAttn {
     bool q_vec, o_vec;            // rows allow 16-byte reads / 4-element writes
     const int* kv_len;
     int H, G;                     // query heads, query heads per KV head
+    unsigned g_magic;             // 2^32 / G + 1 where that gives every quotient of this call (0: divide)
     int max_kv, causal, window;
     float scale_log2e;
     int n_splits, chunk;          // positions per split (multiple of 64)
     int q_tiles;
     bool tile;                    // attn_paged_tile_kernel (host side)
+    bool by_length;               // tile kernel: sessions by falling kv_len
     float *po, *plse;             // n_splits > 1: [split][T][H][D], [split][T][H] (log2 of the sum of exp2)
 };
 
@@ -74,6 +76,16 @@ template <typename F> struct OctetBits {
     __device__ __forceinline__ F keep(const F& f) const { return __builtin_bit_cast(F, __builtin_bit_cast(bits_t, f) & w); }
 };
 
+__device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// new row of column vr (vr >= 0): vr / G
+__device__ __forceinline__ int row_of(const PagedAttn& p, int vr) { return p.G == 1 ? vr : p.g_magic ? (int)__umulhi((unsigned)vr, p.g_magic) : vr / p.G; }
+
 // where the columns of a tile of query rows stand
 struct Span {
     int row0, n;                  // rows of the session
@@ -87,8 +99,7 @@ __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, in
     if (s.n <= 0 || s.row0 >= p.r.T || vr0 >= s.n * p.G) return false;
     s.len = max(0, min(len, p.max_kv));
     s.past = s.len - s.n;
-    const int t0 = vr0 / p.G, t1 = min(vr0 + nvr, s.n * p.G) - 1;
-    const int t_last = t1 / p.G;
+    const int t0 = row_of(p, vr0), t_last = row_of(p, min(vr0 + nvr, s.n * p.G) - 1);
     s.hi = p.causal ? max(0, min(s.len, s.past + t_last + 1)) : s.len;
     s.hi_all = p.causal ? max(0, min(s.len, s.past + t0 + 1)) : s.len;
     s.lo = p.window > 0 ? max(0, s.past + t0 + 1 - p.window) : 0;
@@ -99,54 +110,39 @@ __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, in
 // 4 octets of a query row per 128 channels in the operand's type.  4-bit caches: float16 after dividing the row by a power of two (exact), so that its
 // largest value lies in [1, 2); `mul` gives it back.  bf16 values down to 2^-17 of the largest stay exact, smaller ones are off by at most 2^-25 of it.
 template <int KIND, int D>
-__device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row, bool valid, bool vec, int g, typename KvT<KIND>::frag_t (&q)[D / 32],
-                                           float& mul) {
+__device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row, bool vec, int g, typename KvT<KIND>::frag_t (&q)[D / 32], float& mul) {
     mul = 1.f;
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND == KV_INT4 ? KV_BF16 : KIND>::frag_t raw_t;
-    float x[D / 32][8];
+    raw_t w[D / 32];
+    if (vec) {
 #pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-        raw_t w;
+        for (int s = 0; s < D / 32; ++s) w[s] = *reinterpret_cast<const raw_t*>(row + s * 32 + g * 8);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = 0;
-        if (valid) {
-            if (vec) {
-                w = *reinterpret_cast<const raw_t*>(row + s * 32 + g * 8);
-            } else {
-                T one[8];
+        for (int s = 0; s < D / 32; ++s) {
+            T one[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) one[e] = row[s * 32 + g * 8 + e];
-                __builtin_memcpy(&w, one, sizeof(one));
-            }
+            for (int e = 0; e < 8; ++e) one[e] = row[s * 32 + g * 8 + e];
+            __builtin_memcpy(&w[s], one, sizeof(one));
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[s][e] = (float)w[e];
     }
     if constexpr (KIND == KV_INT4) {
         float m = 0.f;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[s][e]));
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
+            for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)w[s][e]));
+        m = max_over_groups(m);
         const int ex = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
         mul = ldexpf(1.f, ex);
 #pragma unroll
         for (int s = 0; s < D / 32; ++s)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)ldexpf(x[s][e], -ex);
-    } else if constexpr (KIND == KV_BF16) {
-#pragma unroll
-        for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q[s][e] = (__bf16)x[s][e];
+            for (int e = 0; e < 8; ++e) q[s][e] = (_Float16)ldexpf((float)w[s][e], -ex);
     } else {
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q[s][e] = x[s][e];
+        for (int s = 0; s < D / 32; ++s) q[s] = w[s];
     }
 }
 
@@ -327,13 +323,6 @@ constexpr float MAX_SLACK = 8.f;
 constexpr float max_bias(int kind) { return kind == KV_INT4 ? 7.f : 0.f; }
 constexpr float NO_MAX = -3e38f;                  // finite, so that masked scores (-inf) minus it stay -inf
 
-__device__ __forceinline__ float max_over_groups(float x) {        // over the 4 lanes l, l ^ 16, l ^ 32, l ^ 48
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 // scores of a tile -> softmax step and products with the tile's values
 template <int KIND, int D>
 __device__ __forceinline__ void step_tile(const f32x4_t (&s)[tile_u(KIND, D)][2], const ValTile<KIND, D>& vt, const unsigned char* own, int g, float sc, float& m, float& l, f32x4_t (&acc)[D / 16]) {
@@ -406,16 +395,12 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
     const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
     Span sp;
     if (!tile_span(p, b, vr0, 16, sp)) return;
-    const int vr = vr0 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
-    const bool valid = vr < sp.n * p.G;
-    const int c_hi = !valid ? 0 : p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
+    // a column behind the last (row, head) does the last one's work again and stores nothing
+    const bool valid = vr0 + l15 < sp.n * p.G;
+    const int vr = min(vr0 + l15, sp.n * p.G - 1), t = row_of(p, vr), h = hk * p.G + vr - t * p.G;
+    const int c_hi = p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
     const int c_lo = p.window > 0 ? sp.past + t + 1 - p.window : 0;
     const int k0 = (sp.lo & ~63) + split * p.chunk, k1 = min(sp.hi, k0 + p.chunk);
-
-    frag_t q[NS];
-    float sc;
-    load_query<KIND, D>((const T*)p.q + (sp.row0 + t) * p.q_rs + (long)h * D, valid, p.q_vec, g, q, sc);
-    sc *= p.scale_log2e;
 
     f32x4_t acc[ND];
 #pragma unroll
@@ -435,6 +420,10 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
             kt.load(p, head, kb & ps_mask, k_off, lane);
             vt.load(p, head, kb & ps_mask, v_off, m_off);
         }
+        frag_t q[NS];                              // (behind the first tile's loads, so that they are on their way while it is waited for)
+        float sc;
+        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, g, q, sc);
+        sc *= p.scale_log2e;
         for (; kb < k1; kb += W * TK) {
             const int nb = kb + W * TK;
             const long nhead = (long)(page_ok(p.r, next) ? next : 0) * p.r.Hkv + hk;
@@ -705,15 +694,17 @@ __device__ __forceinline__ void tile_step(const unsigned char* buf, const LdsOff
 
 // The session whose kv_len is the i-th largest (up to 64 sessions, a lane each: beyond that there are workgroups enough for the order not to matter).  Long
 // sessions are begun first, so that what is left at the end is short (ragged prompts: 462 -> 437 us; 16 sessions over 4-bit pages, all workgroups resident at once, so
-// that long ones share a CU with short ones: 142 -> 124 us).
+// that long ones share a CU with short ones: 142 -> 124 us).  Ranking takes 0.5 us (8 sessions) to 1.7 us (64): only where it pays, see attn_launch.
 __device__ __forceinline__ int session_by_length(const PagedAttn& p, int i, int lane) {
-    if (p.r.B > 64) return i;
-    const int len = lane < p.r.B ? p.kv_len[lane] : -1;
+    if (!p.by_length) return i;
+    const int len = lane < p.r.B ? max(p.kv_len[lane], 0) : -1;
     int rank = 0;
-    for (int j = 0; j < p.r.B; ++j) {
-        const int other = __builtin_amdgcn_readlane(len, j);
-        rank += other > len || (other == len && j < lane) ? 1 : 0;
-    }
+    for (int j0 = 0; j0 < p.r.B; j0 += 16)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {             // (lanes without a session hold -1: behind all, in lane order)
+            const int other = __builtin_amdgcn_readlane(len, j0 + j);
+            rank += other > len || (other == len && j0 + j < lane) ? 1 : 0;
+        }
     return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(lane < p.r.B && rank == i)) - 1);
 }
 
@@ -744,14 +735,25 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
     const int nvr = sp.n * p.G;
     const int k0 = (sp.lo & ~63) + split * p.chunk, k1 = min(sp.hi, k0 + p.chunk);
 
-    frag_t q[NC][NS];
+    const int ps_mask = (1 << p.r.ps_log2) - 1;
+    int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1, cur = 0;
+    CodeRegs<D> regs;
+    const LdsOff<KIND, D> off(l15, g);
+    const TileDma<KIND == KV_INT4 ? KV_BF16 : KIND, D> dma(tid, p.r.ps_log2);
+    if constexpr (KIND == KV_INT4) {               // codes of tile t + 1 are in registers when tile t is begun
+        if (page_ok(p.r, page)) regs.load(p, page, hk, k0 & ps_mask, tid);
+    } else if (page_ok(p.r, page)) {
+        dma.start(p, lds, page, hk, k0 & ps_mask, wave);
+    }
+
+    frag_t q[NC][NS];                              // (behind the first tile's loads, so that they are on their way while it is waited for)
     float sc[NC], m[NC], l[NC];
     int c_lo[NC], c_hi[NC];
     f32x4_t acc[NC][ND];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int vr = vr0 + wave * RW + c * 16 + l15, t = vr / p.G, h = hk * p.G + vr % p.G;
-        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, vr < nvr, p.q_vec, g, q[c], sc[c]);
+    for (int c = 0; c < NC; ++c) {                 // a column behind the last (row, head) does the last one's work again and stores nothing
+        const int vr = min(vr0 + wave * RW + c * 16 + l15, nvr - 1), t = row_of(p, vr), h = hk * p.G + vr - t * p.G;
+        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, g, q[c], sc[c]);
         sc[c] *= p.scale_log2e;
         c_hi[c] = p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
         c_lo[c] = p.window > 0 ? sp.past + t + 1 - p.window : 0;
@@ -760,20 +762,9 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[c][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-
-    const int ps_mask = (1 << p.r.ps_log2) - 1;
-    int page = k0 < k1 ? page_raw(p.r, b, k0) : -1, next = k0 + TK < k1 ? page_raw(p.r, b, k0 + TK) : -1, cur = 0;
-    CodeRegs<D> regs;
-    const LdsOff<KIND, D> off(l15, g);
-    const TileDma<KIND == KV_INT4 ? KV_BF16 : KIND, D> dma(tid, p.r.ps_log2);
-    if constexpr (KIND == KV_INT4) {               // codes of tile t + 1 are in registers when tile t is begun
-        if (page_ok(p.r, page)) {
-            regs.load(p, page, hk, k0 & ps_mask, tid);
-            regs.store(lds, tid);
-        }
+    if constexpr (KIND == KV_INT4) {
+        if (page_ok(p.r, page)) regs.store(lds, tid);
         if (page_ok(p.r, next)) regs.load(p, next, hk, (k0 + TK) & ps_mask, tid);
-    } else if (page_ok(p.r, page)) {
-        dma.start(p, lds, page, hk, k0 & ps_mask, wave);
     }
     for (int kb = k0; kb < k1; kb += TK) {
         __builtin_amdgcn_s_waitcnt(0);             // this wave's part of the tile has landed (loads to LDS count as loads, not as LDS writes)
@@ -807,7 +798,7 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
         l[c] += __shfl_xor(l[c], 16, 64);
         l[c] += __shfl_xor(l[c], 32, 64);
         if (vr >= nvr) continue;
-        const int t = vr / p.G, h = hk * p.G + vr % p.G;
+        const int t = row_of(p, vr), h = hk * p.G + vr - t * p.G;
         const float inv = l[c] > 0.f ? 1.f / l[c] : 0.f;
         const bool none = l[c] == 0.f;
         const long row = sp.row0 + (long)t;
@@ -891,16 +882,39 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
     pl.q_tiles = cdiv(rows_max, rows);
     const long span = causal && window > 0 ? std::min<long>(max_kv, (long)window + cdiv(rows - 1, G) + 1 + 63) + 63 : max_kv;      // from a multiple of 64
     const long groups = pairs * pl.q_tiles;
-    const long want = std::max<long>(1, (pl.tile ? 512 : 1024) / std::max<long>(1, groups));
-    // a split is a tile for every wave at least; where one split of 256 positions does, the second launch costs more than it saves
-    const int least = pl.tile ? 256 : 4 * 32 * tile_u(paged_kind(kv), kv->head_dim);
-    pl.chunk = span <= 256 ? 256 : std::max(least, cdiv(cdiv(span, want), least) * least);
+    if (pl.tile) {
+        // A split shortens the walk and costs a second launch and f32 partial rows, written and read: the number with the least time wins, in us of 128 rows
+        // of 128 channels.  A tile of 64 positions takes 1.25 (bf16), 1.6 (4 bits), 8.2 (f32); two workgroups on a CU take 1.65 (bf16: 2) times as long where all
+        // sessions have the same length and less in ragged batches, hence 1.5; the join takes 4.3 + 0.03 a workgroup.  Measured for 1 / 2 / 4 / 8 splits: bf16, 64
+        // workgroups, 32 tiles 47 / 34 / 28 / 32; 128 and 32 48 / 40 / 42 / 57; 256 and 8 20 / 37 / 50; 256 and 64 121 / 132, ragged 85 / 75; 4 bits, 128 and
+        // 64 107 / 71 / 62 / 73; 256 and 64 109 / 101, ragged 98 / 79; f32, 64 and 16 147 / 86 / 56 / 57.
+        const float size = (float)(rows * kv->head_dim) / (128 * 128), fill = (float)rows_max / (float)(pl.q_tiles * rows);
+        const int kind = paged_kind(kv);
+        const float tile_us = (kind == KV_F32 ? 8.2f : kind == KV_BF16 ? 1.25f : 1.6f) * size, crowd = 1.5f;
+        const int tiles = std::max(1, cdiv(span, 64));
+        float best = 3e38f;
+        int per = tiles;
+        for (int n = 1; n == 1 || (n * groups <= 512 && 2 * n <= tiles); n *= 2) {
+            const int each = cdiv(tiles, n);
+            const float us = tile_us * (float)each * (n * groups > 256 ? crowd : 1.f) + (n > 1 ? 4.3f + 0.03f * size * fill * (float)(n * groups) : 0.f);
+            if (us < best) best = us, per = each;
+        }
+        pl.chunk = per * 64;
+    } else {
+        const long want = std::max<long>(1, 1024 / std::max<long>(1, groups));
+        // a split is a tile for every wave at least; where one split of 256 positions does, the second launch costs more than it saves
+        const int least = 4 * 32 * tile_u(paged_kind(kv), kv->head_dim);
+        pl.chunk = span <= 256 ? 256 : std::max(least, cdiv(cdiv(span, want), least) * least);
+    }
     pl.n_splits = std::max(1, cdiv(span, pl.chunk));
     if (pl.n_splits == 1) pl.chunk = 1 << 30;
     return pl;
 }
 
-template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, const PagedAttn& p) {
+template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, PagedAttn& p) {
+    // Sessions in the order of their lengths: where CUs get more than one workgroup and walks are long.  us without / with, lengths spread evenly up to the given one:
+    // 512 workgroups, 128 positions 17.5 / 19.2, 512: 28.0 / 29.1, 1024: 39.0 / 38.5 (4 bits 42 / 39), 2048: 73 / 66 (75 / 63); 64 workgroups: 0.3 - 1 slower throughout.
+    p.by_length = p.r.B <= 64 && (long)p.q_tiles * p.n_splits * p.r.Hkv * p.r.B > 256 && std::min(p.max_kv, p.chunk) >= 1024;
     if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
     else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
     if (p.n_splits > 8) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
@@ -950,7 +964,10 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     const int es = kv->dtype == S2S_F32 ? 4 : 2;
     p.q_vec = !((uintptr_t)q & 15) && (q_rs * es) % 16 == 0;
     p.o_vec = !((uintptr_t)o & 15) && (o_rs * es) % 16 == 0;
-    p.H = H; p.G = H / kv->kv_heads; p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
+    p.H = H; p.G = H / kv->kv_heads;
+    // quotients by multiplication: 2^32 / G + 1 is right up to vr G < 2^32
+    p.g_magic = p.G > 1 && (int64_t)p.r.max_new * p.G * p.G < (1LL << 32) ? (unsigned)((1ULL << 32) / p.G + 1) : 0u;
+    p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
     p.scale_log2e = scale * 1.44269504088896340736f;
     p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles; p.tile = pl.tile;
     p.po = (float*)ws_dev;

@@ -328,6 +328,25 @@ def test_attend_many_sessions_with_prompts(kind, dtype):
 
 
 @pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("B,Hkv,new", [(33, 8, 5), (64, 5, 5), (65, 5, 5)])
+def test_attend_ragged_sessions_over_long_tables(kind, dtype, B, Hkv, new):
+    """More workgroups than CUs and tables of 1024 positions and more: sessions are taken by length up to 64 of them, some without rows or positions."""
+    r = random.Random(B)
+    kv = [r.choice([0, 1, 64, 130, 700, 1100]) for _ in range(B - 1)] + [1100]
+    rows = [r.choice([0, 1, new]) for _ in range(B - 1)] + [new]
+    check_attention(rows, kv, Hkv, Hkv * 13, 64, 64, kind, dtype, seed=B, few=False)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("new,kv,Hkv,H,D,ps", [([40], [4100], 1, 2, 64, 64), ([70, 3], [2500, 3], 1, 1, 128, 128), ([35], [1300], 1, 2, 256, 64)])
+def test_attend_few_rows_of_a_long_past_in_splits(kind, dtype, new, kv, Hkv, H, D, ps):
+    """A few tiles of rows over thousands of positions: many splits, some of them behind every row or empty."""
+    check_attention(new, kv, Hkv, H, D, ps, kind, dtype, few=False)
+    check_attention(new, kv, Hkv, H, D, ps, kind, dtype, causal=False, seed=3, few=False, aligned=False, max_kv=-(-max(kv) // ps) * ps)
+    check_attention(new, kv, Hkv, H, D, ps, kind, dtype, window=700, seed=5, few=False)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
 @pytest.mark.parametrize("rows", [17, 24, 32, 33, 64, 65])
 def test_attend_row_counts_around_the_kernels_borders(kind, dtype, rows):
     """(row, head) pairs per KV head at which one kernel hands over to the other, with few and with many sessions."""
