@@ -294,7 +294,7 @@ int32_t s2s_op_kv_read_paged(void* stream, const s2s_paged_kv* kv, const int32_t
 /* o = softmax(scale q k^T) v over the pages, H query heads in H / kv_heads neighbours per KV head.  kv_len_dev int32 [B]: positions in the cache,
  * the new rows' own among them.  causal: new row i of n sees the positions below kv_len - n + i + 1, window > 0 (causal only): the last
  * `window` of those.  A row that sees nothing is zero.  Pages may hold anything (NaN too) at positions at and behind kv_len; positions below it that
- * some row of the call sees hold numbers.  Scores, softmax and sums are f32.
+ * some row of the call sees hold numbers.  Scores, softmax and sums are f32.  scale: any number whose product with log2 e is finite, zero and negative ones too.
  * ws_dev: s2s_op_attn_paged_ws(...) bytes (0: none needed), overwritten; calls that may run at the same time need one each. */
 int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const void* q, int64_t q_rs, void* o, int64_t o_rs, int32_t H, const int32_t* table_dev,
                           int32_t table_cols, const int32_t* kv_len_dev, const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, int32_t max_kv,

@@ -27,7 +27,7 @@ struct PagedAttn {
     int H, G;                     // query heads, query heads per KV head
     unsigned g_magic;             // 2^32 / G + 1 where that gives every quotient of this call (0: divide)
     int max_kv, causal, window;
-    float scale_log2e;
+    float q_mul, scale_log2e;     // the scale times log2 e as a factor of the query rows, -1, 0 or 1, and a positive rest: see score_scale
     int n_splits, chunk;          // positions per split (multiple of 64)
     int q_tiles;
     bool tile;                    // attn_paged_tile_kernel (host side)
@@ -107,10 +107,17 @@ __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, in
     return true;
 }
 
-// 4 octets of a query row per 128 channels in the operand's type.  4-bit caches: float16 after dividing the row by a power of two (exact), so that its
+// A score that a mask hides is -inf before it is scaled, so what scores are multiplied by has to be positive, or -inf would become NaN or +inf: the sign of the
+// scale, or its being zero, goes to the query row, where both are exact and a NaN stays one.  4 bits: the row's power of two times the scale may leave
+// the floats at either end, where it is cut (a positive factor below the smallest normal float makes every score 0 as the float itself does).
+template <int KIND> __device__ __forceinline__ float score_scale(const PagedAttn& p, float mul) {
+    return KIND == KV_INT4 ? fminf(fmaxf(mul * p.scale_log2e, 0x1p-126f), 0x1.fffffep127f) : p.scale_log2e;
+}
+
+// 4 octets of a query row per 128 channels in the operand's type, times q_mul.  4-bit caches: float16 after dividing the row by a power of two (exact), so that its
 // largest value lies in [1, 2); `mul` gives it back.  bf16 values down to 2^-17 of the largest stay exact, smaller ones are off by at most 2^-25 of it.
 template <int KIND, int D>
-__device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row, bool vec, int g, typename KvT<KIND>::frag_t (&q)[D / 32], float& mul) {
+__device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row, bool vec, float q_mul, int g, typename KvT<KIND>::frag_t (&q)[D / 32], float& mul) {
     mul = 1.f;
     typedef typename KvT<KIND>::row_t T;
     typedef typename KvT<KIND == KV_INT4 ? KV_BF16 : KIND>::frag_t raw_t;
@@ -126,6 +133,13 @@ __device__ __forceinline__ void load_query(const typename KvT<KIND>::row_t* row,
             for (int e = 0; e < 8; ++e) one[e] = row[s * 32 + g * 8 + e];
             __builtin_memcpy(&w[s], one, sizeof(one));
         }
+    }
+    if (q_mul != 1.f) {
+        typedef std::remove_reference_t<decltype(w[0][0])> elem_t;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[s][e] = (elem_t)((float)w[s][e] * q_mul);
     }
     if constexpr (KIND == KV_INT4) {
         float m = 0.f;
@@ -422,8 +436,8 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
         }
         frag_t q[NS];                              // (behind the first tile's loads, so that they are on their way while it is waited for)
         float sc;
-        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, g, q, sc);
-        sc *= p.scale_log2e;
+        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, p.q_mul, g, q, sc);
+        sc = score_scale<KIND>(p, sc);
         for (; kb < k1; kb += W * TK) {
             const int nb = kb + W * TK;
             const long nhead = (long)(page_ok(p.r, next) ? next : 0) * p.r.Hkv + hk;
@@ -753,8 +767,8 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
 #pragma unroll
     for (int c = 0; c < NC; ++c) {                 // a column behind the last (row, head) does the last one's work again and stores nothing
         const int vr = min(vr0 + wave * RW + c * 16 + l15, nvr - 1), t = row_of(p, vr), h = hk * p.G + vr - t * p.G;
-        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, g, q[c], sc[c]);
-        sc[c] *= p.scale_log2e;
+        load_query<KIND, D>((const T*)p.q + (sp.row0 + (long)t) * p.q_rs + (long)h * D, p.q_vec, p.q_mul, g, q[c], sc[c]);
+        sc[c] = score_scale<KIND>(p, sc[c]);
         c_hi[c] = p.causal ? min(sp.len, sp.past + t + 1) : sp.len;
         c_lo[c] = p.window > 0 ? sp.past + t + 1 - p.window : 0;
         m[c] = NO_MAX;
@@ -952,6 +966,8 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     if (rc) return rc;
     PagedAttn p{};
     if ((rc = paged_rows(p.r, kv, table_dev, table_cols, cu_dev, B, T, max_new, "attn_paged"))) return rc;
+    const float scale_log2e = fabsf(scale) * 1.44269504088896340736f;
+    S2S_REQUIRE(scale_log2e < INFINITY, "attn_paged: scale %g is not finite in units of log2", (double)scale);       // (NaN too)
     S2S_REQUIRE(max_kv <= table_cols * kv->page_size, "attn_paged: max_kv=%d of %d pages per session", max_kv, table_cols);
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(q && o && kv_len_dev, "attn_paged: null buffer");
@@ -968,7 +984,8 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     // quotients by multiplication: 2^32 / G + 1 is right up to vr G < 2^32
     p.g_magic = p.G > 1 && (int64_t)p.r.max_new * p.G * p.G < (1LL << 32) ? (unsigned)((1ULL << 32) / p.G + 1) : 0u;
     p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
-    p.scale_log2e = scale * 1.44269504088896340736f;
+    p.q_mul = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
+    p.scale_log2e = scale == 0.f ? 1.f : scale_log2e;
     p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles; p.tile = pl.tile;
     p.po = (float*)ws_dev;
     p.plse = p.po + (int64_t)pl.n_splits * T * H * kv->head_dim;

@@ -234,7 +234,7 @@ class PagedKVCache:
 
     def attend(self, q, table, kv_len, cu=None, *, max_new=None, max_kv=None, scale=None, causal: bool = True, window: int = 0, out=None, workspace=None):
         """softmax(scale q k^T) v over the first ``kv_len[b]`` positions of every session (the new rows' own among them) -> ``out`` (new, or given).
-        ``q`` [rows][heads][head_dim], heads a multiple of ``kv_heads``; ``scale`` None: head_dim ** -0.5.  causal: new row i of n sees the positions
+        ``q`` [rows][heads][head_dim], heads a multiple of ``kv_heads``; ``scale`` (any finite number) None: head_dim ** -0.5.  causal: new row i of n sees the positions
         below kv_len - n + i + 1, ``window`` > 0: the last ``window`` of those.  A row that sees nothing is zero.  ``workspace``: uint8 tensor of
         ``workspace_bytes`` (None: taken from torch's allocator; one given to calls on several streams at once would be overwritten)."""
         device, dim = self.device, self.head_dim

@@ -1,0 +1,18 @@
+"""Refusals of the paged cache's operators at the edges of what they take, without a GPU (nothing is launched)."""
+
+import ctypes as C
+import math
+
+import pytest
+
+from speech_to_speech_amd import native
+from test_paged import P, handle
+
+
+def attend(kv, *, scale=1.0, H=4, o_rs=None, cu=0, B=1, T=1, max_new=1, max_kv=512, ws=0, ws_bytes=0):
+    return native.load().s2s_op_attn_paged(None, C.byref(kv), P, H * 128, P, H * 128 if o_rs is None else o_rs, H, P, 8, P, cu, B, T, max_new, max_kv, scale, 1, 0, ws, ws_bytes)
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 3e38])
+def test_scales_that_are_no_numbers_are_refused(scale):
+    assert attend(handle(), scale=scale) == -1 and b"scale" in native.load().s2s_last_error()
