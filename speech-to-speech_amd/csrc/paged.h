@@ -50,17 +50,18 @@ struct PagedRows {
     int B, T, max_new;                // T rows in the row buffers; a session has at most max_new
     int n_pages, ps_log2, Hkv;
 };
-// rows [row0, row0 + n) of session b, cut to the buffers and to max_new
-__device__ __forceinline__ void session_rows(const PagedRows& r, int b, int& row0, int& n) {
+// rows [row0, row0 + n) of session b, cut to the buffers and to max_new -> how many there are uncut
+__device__ __forceinline__ int session_rows(const PagedRows& r, int b, int& row0, int& n) {
     if (!r.cu) {
         row0 = b;
         n = 1;
-        return;
+        return 1;
     }
     const int c0 = r.cu[b], c1 = r.cu[b + 1];
     row0 = max(c0, 0);
     n = min(min(c1, r.T) - row0, r.max_new);
     n = max(n, 0);
+    return c1 - row0;
 }
 // The same number as a scalar load, not yet looked at: the wait for it falls where page_ok asks.  b and pos must be the same in all lanes (the table is
 // only read by these kernels, so the constant address space holds).

@@ -88,21 +88,21 @@ __device__ __forceinline__ int row_of(const PagedAttn& p, int vr) { return p.G =
 
 // where the columns of a tile of query rows stand
 struct Span {
-    int row0, n;                  // rows of the session
-    int len, past;                // positions that count, and before the new rows' own (negative: the first rows see nothing)
-    int lo, hi;                   // positions some row of the tile sees: [lo, hi)
+    int row0, n;                  // rows of the session that are computed
+    int len, past;                // positions that count; positions before the new rows' own (negative: the first rows see nothing).  A session beyond the
+                                  // bounds has fewer rows and positions, but those that are left keep their places: `past` is taken from the uncut numbers
+    int lo, hi;                   // positions some row of the tile sees: [lo, hi); empty where lo >= hi
     int lo_all, hi_all;           // positions every row sees
 };
 __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, int nvr, Span& s) {
-    const int len = p.kv_len[b];
-    session_rows(p.r, b, s.row0, s.n);
+    const int len = max(p.kv_len[b], 0), rows = session_rows(p.r, b, s.row0, s.n);
     if (s.n <= 0 || s.row0 >= p.r.T || vr0 >= s.n * p.G) return false;
-    s.len = max(0, min(len, p.max_kv));
-    s.past = s.len - s.n;
+    s.len = min(len, p.max_kv);
+    s.past = len - rows;
     const int t0 = row_of(p, vr0), t_last = row_of(p, min(vr0 + nvr, s.n * p.G) - 1);
     s.hi = p.causal ? max(0, min(s.len, s.past + t_last + 1)) : s.len;
     s.hi_all = p.causal ? max(0, min(s.len, s.past + t0 + 1)) : s.len;
-    s.lo = p.window > 0 ? max(0, s.past + t0 + 1 - p.window) : 0;
+    s.lo = p.window > 0 ? max(0, min(s.len, s.past + t0 + 1 - p.window)) : 0;
     s.lo_all = p.window > 0 ? max(0, s.past + t_last + 1 - p.window) : 0;
     return true;
 }

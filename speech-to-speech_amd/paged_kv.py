@@ -14,8 +14,8 @@ type or in 4 bits (bf16 models; a scale and a zero per 32 channels of a position
     o = cache.attend(q, table, kv_len + 1, max_kv=longest_session + 1)
 
 Everything is enqueued on torch's current stream of the cache's device and nothing synchronises: ``max_new`` and ``max_kv`` are HOST bounds of
-the device-side lengths (a captured graph replays with other lengths below them).  Sessions longer than the bounds are cut to them.  Tensors
-are containers only; there is no CPU path.
+the device-side lengths (a captured graph replays with other lengths below them).  Of a session beyond the bounds the rows and positions
+beyond are left out; the others keep their places in the session.  Tensors are containers only; there is no CPU path.
 """
 
 from __future__ import annotations

@@ -42,3 +42,55 @@ def test_attend_4_bits_with_queries_near_the_smallest_float(rows, size, scale):
     kd, vd = R.four_bit_values(k).double(), R.four_bit_values(v).double()
     want, weight = R.attend(q.double(), kd, vd, rows, scale)
     assert ((o - want).abs() <= tolerance(want, weight, "int4", BF, float(vd.abs().max()), n, D, False)).all()
+
+
+# ---- sessions beyond the host's bounds --------------------------------------------------------------------------------------------------------
+
+CUTS = [  # new rows, bound of the new rows, positions, bound of the positions, Hkv, H, D, ps
+    ([9, 1, 4], 3, [200, 64, 4], 200, 2, 4, 64, 64),              # single rows' kernel, one walk
+    ([2, 3], 1, [70, 3], 70, 1, 2, 128, 64),
+    ([9, 1], 3, [1500, 64], 1500, 2, 4, 64, 64),                  # a few splits
+    ([9, 2], 3, [4000, 2], 4000, 1, 4, 64, 64),                   # many
+    ([130, 70], 80, [200, 70], 200, 2, 4, 128, 64),               # prompts' kernel
+    ([100, 3], 70, [3000, 5], 3000, 1, 2, 64, 64),                # in splits
+    ([5, 1], 9, [300, 64], 230, 2, 4, 64, 64),                    # more positions than the bound
+    ([9, 40], 7, [300, 100], 64, 1, 4, 64, 64),                   # both; some rows' own positions lie behind the bound
+    ([150, 90], 100, [2900, 800], 2500, 1, 2, 64, 64),
+    ([1, 1], 1, [900, 64], 500, 2, 4, 256, 64),
+]
+
+
+def attend_beyond(kind, dtype, case, causal=True, window=0, rows=None):
+    """-> for every session (what the call gave for its rows, 64 bits of those within the bounds, their tolerance, its rows within the bounds)."""
+    new, max_new, kv, max_kv, Hkv, H, D, ps = case
+    B, cu, starts = len(new), ragged(new), ragged(kv)
+    table, n_pages = make_table(kv, ps, 2, sum(kv))
+    cache = poisoned(n_pages, Hkv, D, ps, kind, dtype)
+    k, v = randn(starts[-1], Hkv, D, seed=1, dtype=dtype), randn(starts[-1], Hkv, D, seed=2, dtype=dtype)
+    cache.append(k.to(DEV), v.to(DEV), table.to(DEV), i32([0] * B), i32(starts), max_new=max(kv))
+    kd, vd = (R.four_bit_values(x).double() for x in (k, v)) if kind == "int4" else (k.double(), v.double())
+    T = cu[-1] if rows is None else rows
+    q, out = randn(cu[-1], H, D, seed=3, dtype=dtype), torch.full((T + 2, H, D), 3.0, dtype=dtype, device=DEV)[:T]
+    cache.attend(q[:T].to(DEV), table.to(DEV), i32(kv), i32(cu), max_new=max_new, max_kv=max_kv, causal=causal, window=window, out=out)
+    got, result = out.cpu().double(), []
+    for b in range(B):
+        vv, r = vd[starts[b] : starts[b + 1]], slice(cu[b], cu[b + 1])
+        want, size = R.attend(q[r].double(), kd[starts[b] : starts[b + 1]], vv, new[b], D**-0.5, causal, window, torch.arange(kv[b]) < max_kv)
+        result.append((got[r], want, tolerance(want, size, kind, dtype, float(vv.abs().max()), kv[b], D, False), min(new[b], max_new, T - cu[b])))
+    return result
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("case", CUTS)
+def test_rows_within_the_bounds_see_what_they_see_without_bounds(kind, dtype, case):
+    """A session with more new rows or positions than the host's bounds: the rows that are computed keep their place in the session."""
+    for mask in (dict(), dict(window=40), dict(causal=False)):
+        for b, (got, want, tol, n) in enumerate(attend_beyond(kind, dtype, case, **mask)):
+            assert ((got[:n] - want[:n]).abs() <= tol[:n]).all(), (mask, b)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_rows_of_a_session_that_ends_behind_the_row_buffer_keep_their_place(kind, dtype):
+    for case, rows in ((([5, 9], 9, [300, 90], 300, 2, 4, 64, 64), 11), (([50, 90], 90, [300, 190], 300, 2, 4, 64, 64), 130)):
+        for got, want, tol, n in attend_beyond(kind, dtype, case, rows=rows):
+            assert ((got[:n] - want[:n]).abs() <= tol[:n]).all()
