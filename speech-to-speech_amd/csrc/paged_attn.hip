@@ -88,17 +88,18 @@ __device__ __forceinline__ int row_of(const PagedAttn& p, int vr) { return p.G =
 
 // where the columns of a tile of query rows stand
 struct Span {
-    int row0, n;                  // rows of the session that are computed
+    int row0, n, rows;            // rows of the session that are computed, and uncut
     int len, past;                // positions that count; positions before the new rows' own (negative: the first rows see nothing).  A session beyond the
                                   // bounds has fewer rows and positions, but those that are left keep their places: `past` is taken from the uncut numbers
     int lo, hi;                   // positions some row of the tile sees: [lo, hi); empty where lo >= hi
     int lo_all, hi_all;           // positions every row sees
 };
 __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, int nvr, Span& s) {
-    const int len = max(p.kv_len[b], 0), rows = session_rows(p.r, b, s.row0, s.n);
+    const int len = max(p.kv_len[b], 0);
+    s.rows = session_rows(p.r, b, s.row0, s.n);
     if (s.n <= 0 || s.row0 >= p.r.T || vr0 >= s.n * p.G) return false;
     s.len = min(len, p.max_kv);
-    s.past = len - rows;
+    s.past = len - s.rows;
     const int t0 = row_of(p, vr0), t_last = row_of(p, min(vr0 + nvr, s.n * p.G) - 1);
     s.hi = p.causal ? max(0, min(s.len, s.past + t_last + 1)) : s.len;
     s.hi_all = p.causal ? max(0, min(s.len, s.past + t0 + 1)) : s.len;
@@ -112,6 +113,13 @@ __device__ __forceinline__ bool tile_span(const PagedAttn& p, int b, int vr0, in
 // the floats at either end, where it is cut (a positive factor below the smallest normal float makes every score 0 as the float itself does).
 template <int KIND> __device__ __forceinline__ float score_scale(const PagedAttn& p, float mul) {
     return KIND == KV_INT4 ? fminf(fmaxf(mul * p.scale_log2e, 0x1p-126f), 0x1.fffffep127f) : p.scale_log2e;
+}
+
+// Rows of a session beyond max_new get no partial results.  The join, which goes by rows, leaves out those whose weight in split 0 is +inf, which no result is (a
+// maximum of +inf comes with a NaN or an empty sum): one workgroup of the session puts it there.
+__device__ __forceinline__ void leave_rows(const PagedAttn& p, const Span& s) {
+    const long end = min((long)s.row0 + s.rows, (long)p.r.T) * p.H;
+    for (long i = ((long)s.row0 + s.n) * p.H + threadIdx.x; i < end; i += 256) p.plse[i] = INFINITY;
 }
 
 // 4 octets of a query row per 128 channels in the operand's type, times q_mul.  4-bit caches: float16 after dividing the row by a power of two (exact), so that its
@@ -409,6 +417,7 @@ __global__ __launch_bounds__(256, KIND == KV_INT4 ? (D == 64 ? 4 : D == 128 ? 3 
     const int b = blockIdx.z, hk = blockIdx.y, split = blockIdx.x % p.n_splits, vr0 = (blockIdx.x / p.n_splits) * 16;
     Span sp;
     if (!tile_span(p, b, vr0, 16, sp)) return;
+    if (p.n_splits > 1 && blockIdx.x == 0 && hk == 0) leave_rows(p, sp);
     // a column behind the last (row, head) does the last one's work again and stores nothing
     const bool valid = vr0 + l15 < sp.n * p.G;
     const int vr = min(vr0 + l15, sp.n * p.G - 1), t = row_of(p, vr), h = hk * p.G + vr - t * p.G;
@@ -745,6 +754,7 @@ __global__ __launch_bounds__(256, D == 256 && KIND == KV_F32 ? 1 : 2) void attn_
     const int b = session_by_length(p, pair / p.r.Hkv, lane), hk = pair % p.r.Hkv, split = w % p.n_splits, vr0 = (p.q_tiles - 1 - w / p.n_splits) * 4 * RW;
     Span sp, sw;
     if (!tile_span(p, b, vr0, 4 * RW, sp)) return;
+    if (p.n_splits > 1 && vr0 == 0 && split == 0 && hk == 0) leave_rows(p, sp);
     if (!tile_span(p, b, vr0 + wave * RW, RW, sw)) sw.lo = sw.hi = sw.lo_all = sw.hi_all = 0;      // no rows: help with the tiles only
     const int nvr = sp.n * p.G;
     const int k0 = (sp.lo & ~63) + split * p.chunk, k1 = min(sp.hi, k0 + p.chunk);
@@ -846,6 +856,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn p) {
     float M = NO_MAX;
     for (int s = lane; s < p.n_splits; s += 64) M = fmaxf(M, p.plse[s * n + i]);
     M = wave_max(M);
+    if (M == INFINITY) return;              // not computed: see leave_rows (the same in all waves of a row)
     float acc[E], L = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;

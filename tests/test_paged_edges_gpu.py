@@ -94,3 +94,11 @@ def test_rows_of_a_session_that_ends_behind_the_row_buffer_keep_their_place(kind
     for case, rows in ((([5, 9], 9, [300, 90], 300, 2, 4, 64, 64), 11), (([50, 90], 90, [300, 190], 300, 2, 4, 64, 64), 130)):
         for got, want, tol, n in attend_beyond(kind, dtype, case, rows=rows):
             assert ((got[:n] - want[:n]).abs() <= tol[:n]).all()
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("case", CUTS)
+def test_rows_beyond_the_bound_are_left_as_they_are(kind, dtype, case):
+    for mask in (dict(), dict(window=40), dict(causal=False)):
+        for b, (got, _, _, n) in enumerate(attend_beyond(kind, dtype, case, **mask)):
+            assert (got[n:] == 3).all(), (mask, b)
