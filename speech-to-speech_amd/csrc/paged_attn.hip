@@ -994,7 +994,7 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     p.H = H; p.G = H / kv->kv_heads;
     // quotients by multiplication: 2^32 / G + 1 is right up to vr G < 2^32
     p.g_magic = p.G > 1 && (int64_t)p.r.max_new * p.G * p.G < (1LL << 32) ? (unsigned)((1ULL << 32) / p.G + 1) : 0u;
-    p.max_kv = max_kv; p.causal = causal != 0; p.window = window;
+    p.max_kv = max_kv; p.causal = causal != 0; p.window = std::min(window, 1 << 30);      // no cache is longer, and differences stay inside 32 bits
     p.q_mul = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
     p.scale_log2e = scale == 0.f ? 1.f : scale_log2e;
     p.n_splits = pl.n_splits; p.chunk = pl.chunk; p.q_tiles = pl.q_tiles; p.tile = pl.tile;

@@ -102,3 +102,25 @@ def test_rows_beyond_the_bound_are_left_as_they_are(kind, dtype, case):
     for mask in (dict(), dict(window=40), dict(causal=False)):
         for b, (got, _, _, n) in enumerate(attend_beyond(kind, dtype, case, **mask)):
             assert (got[n:] == 3).all(), (mask, b)
+
+
+# ---- the C entry points -------------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("new,kv", [(9, 3), (130, 100), (1, 64)])
+def test_a_window_of_the_largest_integer_hides_nothing(new, kv):
+    """Also for rows in front of the first position."""
+    Hkv, H, D = 1, 2, 64
+    table, n_pages = make_table([kv], 64, 0, 1)
+    tb = table.to(DEV)
+    cache = poisoned(n_pages, Hkv, D, 64, "model", F32)
+    cache.append(randn(kv, Hkv, D, seed=1).to(DEV), randn(kv, Hkv, D, seed=2).to(DEV), tb, i32([0]), i32([0, kv]), max_new=kv)
+    q, lens, cu = randn(new, H, D, seed=3).to(DEV), i32([kv]), i32([0, new])
+    outs = []
+    for window in (1 << 29, 2**31 - 1):
+        out = torch.full_like(q, 3.0)
+        st = native.load().s2s_op_attn_paged(torch.cuda.current_stream().cuda_stream, C.byref(cache._kv), q.data_ptr(), H * D, out.data_ptr(), H * D, H, tb.data_ptr(), tb.shape[1],
+                                             lens.data_ptr(), cu.data_ptr(), 1, new, new, kv, 0.125, 1, window, 0, 0)
+        assert st == 0, native.load().s2s_last_error()
+        outs.append(out)
+    assert torch.equal(*outs) and float(outs[0][-1].abs().max()) > 0
