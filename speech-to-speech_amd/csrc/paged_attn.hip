@@ -936,13 +936,15 @@ static PagedPlan paged_plan(const s2s_paged_kv* kv, int H, int B, int max_new, i
     return pl;
 }
 
+constexpr int64_t MAX_GROUPS = 1 << 24;       // a launch has fewer than 2^32 work-items along a dimension
+
 template <typename T, int KIND, int D> static void attn_launch(hipStream_t st, PagedAttn& p) {
     // Sessions in the order of their lengths: where CUs get more than one workgroup and walks are long.  us without / with, lengths spread evenly up to the given one:
     // 512 workgroups, 128 positions 17.5 / 19.2, 512: 28.0 / 29.1, 1024: 39.0 / 38.5 (4 bits 42 / 39), 2048: 73 / 66 (75 / 63); 64 workgroups: 0.3 - 1 slower throughout.
     p.by_length = p.r.B <= 64 && (long)p.q_tiles * p.n_splits * p.r.Hkv * p.r.B > 256 && std::min(p.max_kv, p.chunk) >= 1024;
     if (p.tile) attn_paged_tile_kernel<KIND, D, tile_nc(D)><<<dim3(p.q_tiles * p.n_splits * p.r.Hkv * p.r.B), 256, 0, st>>>(p);
     else attn_paged_step_kernel<KIND, D><<<dim3(p.q_tiles * p.n_splits, p.r.Hkv, p.r.B), 256, 0, st>>>(p);
-    if (p.n_splits > 8) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
+    if (p.n_splits > 8 && (long)p.r.T * p.H < MAX_GROUPS) attn_paged_join_kernel<T, D, 4><<<dim3(p.r.T * p.H), 256, 0, st>>>(p);
     else if (p.n_splits > 1) attn_paged_join_kernel<T, D, 1><<<cdiv((long)p.r.T * p.H, 4), 256, 0, st>>>(p);
 }
 
@@ -959,7 +961,9 @@ static int attn_paged_sizes(const s2s_paged_kv* kv, int H, int B, int T, int max
     S2S_REQUIRE((int64_t)T * H < (1LL << 31), "attn_paged: %d rows of %d heads are too many for one call", T, H);
     if (B == 0 || T == 0) return S2S_OK;
     const PagedPlan pl = paged_plan(kv, H, B, std::min(max_new, T), max_kv, causal, window);
-    S2S_REQUIRE((int64_t)pl.q_tiles * pl.n_splits * kv->kv_heads * B < (1LL << 31), "attn_paged: %d sessions of up to %d rows are too many for one call", B, max_new);
+    const int64_t groups = (int64_t)pl.q_tiles * pl.n_splits * (pl.tile ? (int64_t)kv->kv_heads * B : 1);     // (the step kernel's heads and sessions lie along others)
+    S2S_REQUIRE(groups < MAX_GROUPS, "attn_paged: %d sessions of up to %d rows are too many for one call", B, max_new);
+    S2S_REQUIRE(pl.n_splits == 1 || cdiv((int64_t)T * H, 4) < MAX_GROUPS, "attn_paged: %d rows of %d heads are too many for one call", T, H);
     return S2S_OK;
 }
 
