@@ -40,6 +40,8 @@ __device__ __forceinline__ void codes_to_f16(unsigned w, f16x2_t (&c)[4]) {
 // fields of a packed cache handle, checked by paged_check (paged.hip)
 int paged_check(const s2s_paged_kv* kv, const char* who);
 struct PagedRows;
+// rows [T][n elements] that are written, rs apart: no two share memory
+inline bool rows_apart(int T, int64_t rs, int64_t n) { return T <= 1 || rs >= n; }
 int paged_rows(PagedRows& r, const s2s_paged_kv* kv, const int* table, int cols, const int* cu, int B, int T, int max_new, const char* who);
 inline int paged_kind(const s2s_paged_kv* kv) { return kv->kind == S2S_KV_INT4 ? KV_INT4 : kv->dtype == S2S_F32 ? KV_F32 : KV_BF16; }
 

@@ -726,6 +726,10 @@ extern "C" int32_t s2s_op_rope(void* stream, const void* x, int64_t x_rs, int64_
     S2S_REQUIRE(x != out || (x_rs == o_rs && x_hs == o_hs), "rope: in place needs the same strides");
     if (rows == 0 || heads == 0) return S2S_OK;
     S2S_REQUIRE(x && out && positions_dev, "rope: null buffer");
+    // heads inside rows, or rows inside heads
+    S2S_REQUIRE((rows_apart(heads, o_hs, head_dim) && rows_apart(rows, o_rs, (heads - 1) * o_hs + head_dim)) ||
+                    (rows_apart(rows, o_rs, head_dim) && rows_apart(heads, o_hs, (rows - 1) * o_rs + head_dim)),
+                "rope: rows of out share memory (strides %lld, %lld)", (long long)o_rs, (long long)o_hs);
     const int es = dtype == S2S_F32 ? 4 : 2;
     // octets need 16-byte rows and heads, and a rotation that falls on octets in both halves
     const bool vec = rotary_dim % 16 == 0 && head_dim % 8 == 0 && aligned(x, x_rs, es) && aligned(out, o_rs, es) && (x_hs * es) % 16 == 0 && (o_hs * es) % 16 == 0 &&
@@ -761,6 +765,7 @@ extern "C" int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, 
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(k && v && start_dev, "kv_append_paged: null buffer");
     S2S_REQUIRE(q != q_out || q_rs == qo_rs, "kv_append_paged: in place needs the same stride");
+    S2S_REQUIRE(!q || rows_apart(T, qo_rs, (int64_t)H * kv->head_dim), "kv_append_paged: rows of q_out share memory (stride %lld)", (long long)qo_rs);
     const int es = kv->dtype == S2S_F32 ? 4 : 2;
     const bool vec = aligned(k, k_rs, es) && aligned(v, v_rs, es) && (!q || (aligned(q, q_rs, es) && aligned(q_out, qo_rs, es))) &&
                      (!cos_dev || (rotary_dim % 16 == 0 && aligned(cos_dev, 0, 4) && aligned(sin_dev, 0, 4)));
@@ -782,6 +787,7 @@ extern "C" int32_t s2s_op_kv_read_paged(void* stream, const s2s_paged_kv* kv, co
     if ((rc = paged_rows(p.r, kv, table_dev, table_cols, cu_dev, B, T, max_new, "kv_read_paged"))) return rc;
     if (B == 0 || T == 0 || (!k_out && !v_out)) return S2S_OK;
     S2S_REQUIRE(start_dev, "kv_read_paged: null buffer");
+    S2S_REQUIRE(rows_apart(T, o_rs, (int64_t)kv->kv_heads * kv->head_dim), "kv_read_paged: rows share memory (stride %lld)", (long long)o_rs);
     const int es = kv->dtype == S2S_F32 ? 4 : 2;
     const bool vec = (!k_out || aligned(k_out, o_rs, es)) && (!v_out || aligned(v_out, o_rs, es));
     p.kc = kv->k; p.vc = kv->v; p.km = (const _Float16*)kv->k_meta; p.vm = (const _Float16*)kv->v_meta;

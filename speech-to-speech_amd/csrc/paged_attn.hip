@@ -986,6 +986,7 @@ extern "C" int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const
     S2S_REQUIRE(max_kv <= table_cols * kv->page_size, "attn_paged: max_kv=%d of %d pages per session", max_kv, table_cols);
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(q && o && kv_len_dev, "attn_paged: null buffer");
+    S2S_REQUIRE(rows_apart(T, o_rs, (int64_t)H * kv->head_dim), "attn_paged: rows of o share memory (stride %lld)", (long long)o_rs);
     const PagedPlan pl = paged_plan(kv, H, B, p.r.max_new, max_kv, causal, window);
     const int64_t need = pl.n_splits == 1 ? 0 : (int64_t)pl.n_splits * T * H * (kv->head_dim + 1) * 4;
     S2S_REQUIRE(need == 0 || (ws_dev && ws_bytes >= need && !((uintptr_t)ws_dev & 15)), "attn_paged: workspace of %lld bytes, 16-byte aligned, needed (got %lld)",

@@ -116,7 +116,7 @@ def _tables(cos, sin, device):
 
 def rope(x, positions, cos, sin, *, interleaved: bool = False, out=None):
     """Turn the first ``2 * cos.shape[1]`` channels of every head of ``x`` [rows][heads][dim] to its row's position -> ``out`` (new, or given, or
-    ``x`` itself).  ``positions`` int32 [rows]: a negative one leaves the row of ``out`` as it is, one behind the table gives NaN."""
+    ``x`` itself; else they share no memory).  ``positions`` int32 [rows]: a negative one leaves the row of ``out`` as it is, one behind the table gives NaN."""
     device, shape = x.device, x.shape
     if len(shape) != 3 or (x.stride(2) != 1 and x.numel()):
         raise ValueError(f"x: [rows][heads][dim] with neighbouring channels needed, got {tuple(shape)}, strides {x.stride()}")

@@ -30,3 +30,19 @@ def test_more_workgroups_than_a_launch_takes_are_refused():
     one = handle(kv_heads=1)
     assert lib.s2s_op_attn_paged_ws(C.byref(one), 64, 1, 2**19, 1, 2**20, 1, 0) > 0
     assert lib.s2s_op_attn_paged_ws(C.byref(one), 64, 1, 2**20, 1, 2**20, 1, 0) == -1 and b"too many" in lib.s2s_last_error()
+
+
+def test_outputs_whose_rows_share_memory_are_refused():
+    """Two rows (or heads) written to one place would leave whichever came last."""
+    lib, kv, ref = native.load(), handle(), lambda: native.load().s2s_last_error()
+    rope = lambda o_rs, o_hs, rows=3, heads=2: lib.s2s_op_rope(None, P, 128, 64, 2 * P, o_rs, o_hs, P, P, P, 5, rows, heads, 64, 64, 0, 0)  # noqa: E731
+    for o_rs, o_hs in ((0, 64), (127, 64), (128, 0), (128, 63), (64, 191), (63, 192), (-64, 64)):
+        assert rope(o_rs, o_hs) == -1 and b"share" in ref(), (o_rs, o_hs)
+    for o_rs, o_hs, rows, heads in ((0, 0, 2, 1), (63, 0, 2, 1), (0, 63, 1, 2)):
+        assert rope(o_rs, o_hs, rows, heads) == -1 and b"share" in ref(), (o_rs, o_hs, rows, heads)
+    assert lib.s2s_op_rope(None, P, 0, 64, P, 0, 64, P, P, P, 5, 3, 2, 64, 64, 0, 0) == -1 and b"share" in ref()      # a broadcast row turned in place
+    for o_rs in (0, 511, -512):
+        assert attend(kv, cu=P, T=2, max_new=2, o_rs=o_rs) == -1 and b"share" in ref()
+    for o_rs in (0, 255, -256):
+        assert lib.s2s_op_kv_read_paged(None, C.byref(kv), P, 8, P, P, 1, 2, 2, P, P, o_rs) == -1 and b"share" in ref()
+        assert lib.s2s_op_kv_append_paged(None, C.byref(kv), P, 256, P, 256, P, 256, 2 * P, o_rs, 2, P, 8, P, P, 1, 2, 2, P, P, 5, 128, 0) == -1 and b"share" in ref()
