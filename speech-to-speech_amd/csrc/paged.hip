@@ -764,7 +764,7 @@ extern "C" int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, 
     S2S_REQUIRE(!q || (cos_dev && q_out && H >= 1 && H <= 4096), "kv_append_paged: queries need tables, q_out and 1 .. 4096 heads (H=%d)", H);
     if (B == 0 || T == 0) return S2S_OK;
     S2S_REQUIRE(k && v && start_dev, "kv_append_paged: null buffer");
-    S2S_REQUIRE(q != q_out || q_rs == qo_rs, "kv_append_paged: in place needs the same stride");
+    S2S_REQUIRE(!q || q != q_out || q_rs == qo_rs, "kv_append_paged: in place needs the same stride");
     S2S_REQUIRE(!q || rows_apart(T, qo_rs, (int64_t)H * kv->head_dim), "kv_append_paged: rows of q_out share memory (stride %lld)", (long long)qo_rs);
     const int es = kv->dtype == S2S_F32 ? 4 : 2;
     const bool vec = aligned(k, k_rs, es) && aligned(v, v_rs, es) && (!q || (aligned(q, q_rs, es) && aligned(q_out, qo_rs, es))) &&

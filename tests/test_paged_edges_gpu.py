@@ -124,3 +124,13 @@ def test_a_window_of_the_largest_integer_hides_nothing(new, kv):
         assert st == 0, native.load().s2s_last_error()
         outs.append(out)
     assert torch.equal(*outs) and float(outs[0][-1].abs().max()) > 0
+
+
+def test_an_append_without_queries_takes_any_stride_of_theirs():
+    cache, other = (poisoned(2, 1, 64, 64, "model", F32) for _ in range(2))
+    k, v, table, start = randn(2, 1, 64, seed=1).to(DEV), randn(2, 1, 64, seed=2).to(DEV), i32([[0], [1]]), i32([3, 5])
+    cache.append(k, v, table, start)
+    st = native.load().s2s_op_kv_append_paged(torch.cuda.current_stream().cuda_stream, C.byref(other._kv), k.data_ptr(), 64, v.data_ptr(), 64, 0, 7, 0, 64, 0, table.data_ptr(), 1,
+                                              start.data_ptr(), 0, 2, 2, 1, 0, 0, 0, 0, 0)
+    assert st == 0, native.load().s2s_last_error()
+    assert torch.equal(cache.k.view(torch.uint8), other.k.view(torch.uint8)) and torch.equal(cache.v.view(torch.uint8), other.v.view(torch.uint8))
