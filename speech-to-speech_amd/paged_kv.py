@@ -174,7 +174,7 @@ class PagedKVCache:
         self._ws: dict = {}  # workspace bytes by the sizes of a call
 
     def _sessions(self, table, lens, cu, rows, max_new, what):
-        """-> (sessions, pages per session, bound of the new rows)."""
+        """-> (sessions, pages per session, rows, bound of a session's new rows): no rows where the bound leaves none."""
         if table.dtype is not torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.device != self.device:
             raise ValueError(f"table: contiguous int32 [sessions][pages] on {self.device} needed, got {table.dtype} {tuple(table.shape)} on {table.device}")
         b, cols = table.shape
@@ -182,9 +182,13 @@ class PagedKVCache:
         if cu is None:
             if rows != b or max_new not in (None, 1):
                 raise ValueError(f"without cu there is one row per session ({rows} rows, {b} sessions, max_new {max_new})")
-            return b, cols, 1
+            return b, cols, rows, 1
         _ints(cu, b + 1, self.device, "cu")
-        return b, cols, max(1, rows if max_new is None else min(max_new, rows))
+        if max_new is None or max_new > rows:
+            max_new = rows
+        elif max_new < 0:
+            raise ValueError(f"max_new: a number of rows needed, got {max_new}")
+        return (b, cols, rows, max_new) if max_new else (b, cols, 0, 1)
 
     def append(self, k, v, table, start, cu=None, *, max_new=None, cos=None, sin=None, interleaved: bool = False, q=None, q_out=None):
         """Store every session's new rows behind the ``start`` positions its pages hold, keys turned to their positions (``cos`` / ``sin`` None: as they come).
@@ -192,7 +196,7 @@ class PagedKVCache:
         device, dim, dtype = self.device, self.head_dim, self.dtype
         T, _, k_rs = _rows(k, self.kv_heads, dim, dtype, device, "k")
         Tv, _, v_rs = _rows(v, self.kv_heads, dim, dtype, device, "v")
-        b, cols, max_new = self._sessions(table, start, cu, T, max_new, "start")
+        b, cols, rows, max_new = self._sessions(table, start, cu, T, max_new, "start")
         n, rot, cp, sp = (0, 0, 0, 0) if cos is None and sin is None else _tables(cos, sin, device)
         Tq, H, q_rs, qp, qo_rs, qop = T, 0, 0, 0, 0, 0
         if q is not None:
@@ -209,7 +213,7 @@ class PagedKVCache:
         if Tv != T or Tq != T:
             raise ValueError(f"k, v and q need the same rows, got {T}, {Tv} and {Tq}")
         _call(device, "s2s_op_kv_append_paged", native.load().s2s_op_kv_append_paged, self._ref, k.data_ptr(), k_rs, v.data_ptr(), v_rs, qp, q_rs, qop, qo_rs, H, table.data_ptr(), cols,
-              start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, T, max_new, cp, sp, n, rot, 1 if interleaved else 0)
+              start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, rows, max_new, cp, sp, n, rot, 1 if interleaved else 0)
         return q_out if H else None
 
     def read(self, table, start, cu=None, rows=None, *, max_new=None):
@@ -218,8 +222,8 @@ class PagedKVCache:
         if rows is None:
             _require(cu is None, "rows: how many rows cu counts")
             rows = table.shape[0]
-        b, cols, max_new = self._sessions(table, start, cu, rows, max_new, "start")
         shape = (rows, self.kv_heads, self.head_dim)
+        b, cols, rows, max_new = self._sessions(table, start, cu, rows, max_new, "start")
         k, v = torch.empty(shape, dtype=self.dtype, device=self.device), torch.empty(shape, dtype=self.dtype, device=self.device)
         _call(self.device, "s2s_op_kv_read_paged", native.load().s2s_op_kv_read_paged, self._ref, table.data_ptr(), cols, start.data_ptr(), 0 if cu is None else cu.data_ptr(), b, rows,
               max_new, k.data_ptr(), v.data_ptr(), self.kv_heads * self.head_dim)
@@ -239,7 +243,7 @@ class PagedKVCache:
         ``workspace_bytes`` (None: taken from torch's allocator; one given to calls on several streams at once would be overwritten)."""
         device, dim = self.device, self.head_dim
         T, H, q_rs = _rows(q, None, dim, self.dtype, device, "q")
-        b, cols, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
+        b, cols, rows, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
         if max_kv is None:
             max_kv = cols * self.page_size
         elif not 0 <= max_kv <= cols * self.page_size:
@@ -253,10 +257,10 @@ class PagedKVCache:
                 raise ValueError(f"out: {T} rows needed, got {To}")
         c = 1 if causal else 0
         if workspace is None:
-            sizes = (H, b, T, max_new, max_kv, c, window)
+            sizes = (H, b, rows, max_new, max_kv, c, window)
             need = self._ws.get(sizes)
             if need is None:
-                need = self.workspace_bytes(H, b, T, max_new=max_new, max_kv=max_kv, causal=causal, window=window)
+                need = self.workspace_bytes(H, b, rows, max_new=max_new, max_kv=max_kv, causal=causal, window=window)
                 if len(self._ws) >= 4096:
                     self._ws.clear()
                 self._ws[sizes] = need
@@ -266,5 +270,5 @@ class PagedKVCache:
             raise ValueError(f"workspace: contiguous on {device} needed")
         ws, ws_bytes = (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
         _call(device, "s2s_op_attn_paged", native.load().s2s_op_attn_paged, self._ref, q.data_ptr(), q_rs, out.data_ptr(), o_rs, H, table.data_ptr(), cols, kv_len.data_ptr(),
-              0 if cu is None else cu.data_ptr(), b, T, max_new, max_kv, dim ** -0.5 if scale is None else scale, c, window, ws, ws_bytes)
+              0 if cu is None else cu.data_ptr(), b, rows, max_new, max_kv, dim ** -0.5 if scale is None else scale, c, window, ws, ws_bytes)
         return out

@@ -4,8 +4,10 @@ import ctypes as C
 import math
 
 import pytest
+import torch
 
 from speech_to_speech_amd import native
+from speech_to_speech_amd.paged_kv import PagedKVCache
 from test_paged import P, handle
 
 
@@ -46,3 +48,11 @@ def test_outputs_whose_rows_share_memory_are_refused():
     for o_rs in (0, 255, -256):
         assert lib.s2s_op_kv_read_paged(None, C.byref(kv), P, 8, P, P, 1, 2, 2, P, P, o_rs) == -1 and b"share" in ref()
         assert lib.s2s_op_kv_append_paged(None, C.byref(kv), P, 256, P, 256, P, 256, 2 * P, o_rs, 2, P, 8, P, P, 1, 2, 2, P, P, 5, 128, 0) == -1 and b"share" in ref()
+
+
+def test_negative_bounds_are_refused():
+    cache = PagedKVCache(4, 2, 64, device="cpu")
+    table, lens, cu, rows = torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: cache.append(rows, rows, table, lens, cu, max_new=-1), lambda: cache.read(table, lens, cu, 2, max_new=-1), lambda: cache.attend(rows, table, lens, cu, max_new=-1)):
+        with pytest.raises(ValueError, match="max_new"):
+            call()

@@ -8,6 +8,7 @@ import torch
 
 import paged_reference as R
 from speech_to_speech_amd import native
+from speech_to_speech_amd.paged_kv import rope_tables
 from test_paged_gpu import BF, DEV, F32, KINDS, check_attention, i32, make_table, poisoned, ragged, randn, tolerance
 
 pytestmark = pytest.mark.gpu
@@ -134,3 +135,16 @@ def test_an_append_without_queries_takes_any_stride_of_theirs():
                                               start.data_ptr(), 0, 2, 2, 1, 0, 0, 0, 0, 0)
     assert st == 0, native.load().s2s_last_error()
     assert torch.equal(cache.k.view(torch.uint8), other.k.view(torch.uint8)) and torch.equal(cache.v.view(torch.uint8), other.v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_a_bound_of_no_new_rows_leaves_everything_as_it_is(kind, dtype):
+    cache = poisoned(4, 2, 64, 64, kind, dtype)
+    before = [t.clone() for t in (cache.k, cache.v)]
+    rows, table, start, cu = randn(3, 2, 64, seed=1, dtype=dtype).to(DEV), i32([[0, 1], [2, 3]]), i32([3, 64]), i32([0, 1, 3])
+    cos, sin = rope_tables(64, 128, device=DEV)
+    out = torch.full_like(rows, 7.0)
+    assert cache.append(rows, rows, table, start, cu, max_new=0, cos=cos, sin=sin, q=rows, q_out=out) is out
+    assert cache.attend(rows, table, start, cu, max_new=0, out=out) is out
+    assert all(x.shape == rows.shape for x in cache.read(table, start, cu, 3, max_new=0))
+    assert (out == 7).all() and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, (cache.k, cache.v)))
