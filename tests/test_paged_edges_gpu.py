@@ -213,3 +213,43 @@ def test_single_rows_kernel_keeps_what_the_first_rounding_of_a_weight_leaves(row
             once = (p / p.amax(-1, keepdim=True)).to(BF).double()
             off = (once @ vv[:, 0] / (p / p.amax(-1, keepdim=True)).sum(-1, keepdim=True) - want[:, 0]).abs()
             assert (off > tol[:, 0]).any()
+
+
+# ---- what stands together in one call -----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_single_rows_beside_a_prompt(kind, dtype):
+    """The usual batch of a serving loop: a prompt joins sessions that are taking single steps."""
+    kv = [1 + 37 * i % 700 for i in range(47)]
+    check_attention([1] * 23 + [300] + [1] * 24, kv[:23] + [410] + kv[23:], 2, 4, 64, 64, kind, dtype, few=False)
+    check_attention([1] * 8 + [70, 130], kv[:8] + [1500, 130], 1, 2, 128, 64, kind, dtype, few=False, seed=3)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("new,kv,at", [(1, 70, 5), (70, 70, 30), (3, 2100, 2098), (90, 2600, 2550), (90, 2600, 100)])
+def test_an_infinite_score_is_nan_where_it_is_seen_and_nothing_elsewhere(kind, dtype, new, kv, at):
+    """exp(inf - inf) is NaN for the rows that see the key (a 4-bit group with an infinity holds NaN).  Rows before it stay within the tolerance of the call without it: a
+    wave raises the running maxima of its 16 or 32 columns together, at other tiles then, so each weight is a multiple of another 2^-m before it is rounded and
+    what `tolerance` counts is the same.  Another session is bit for bit what it was."""
+    Hkv, H, D, ps = 1, 2, 64, 64
+    table, n_pages = make_table([kv, kv], ps, 0, kv)
+    cache = poisoned(n_pages, Hkv, D, ps, kind, dtype)
+    k, v = randn(2 * kv, Hkv, D, seed=1, dtype=dtype), randn(2 * kv, Hkv, D, seed=2, dtype=dtype)
+    q = randn(2 * new, H, D, seed=3, dtype=dtype)
+    q[..., 7] = 1.0
+    plain = k.clone()
+    k[at, 0, 7] = float("inf")
+    outs = []
+    for rows in (plain, k):
+        cache.append(rows.to(DEV), v.to(DEV), table.to(DEV), i32([0, 0]), i32([0, kv, 2 * kv]), max_new=kv)
+        outs.append(cache.attend(q.to(DEV), table.to(DEV), i32([kv, kv]), i32([0, new, 2 * new]), max_new=new, max_kv=kv).cpu())
+    blind = max(0, at - (kv - new))      # rows of the first session that do not see the key
+    assert torch.isnan(outs[1][blind:new]).all() and torch.isfinite(outs[0]).all()
+    assert torch.equal(outs[1][new:], outs[0][new:])
+    kd, vd = (R.four_bit_values(x[:kv]).double() for x in (plain, v)) if kind == "int4" else (plain[:kv].double(), v[:kv].double())
+    want, size = R.attend(q[:new].double(), kd, vd, new, D**-0.5)
+    tol = tolerance(want, size, kind, dtype, float(vd.abs().max()), kv, D, False)
+    for o in outs:
+        n = new if o is outs[0] else blind
+        assert ((o[:n].double() - want[:n]).abs() <= tol[:n]).all()
