@@ -288,14 +288,16 @@ int32_t s2s_op_kv_append_paged(void* stream, const s2s_paged_kv* kv, const void*
                                int32_t rotary_dim, int32_t interleaved);
 
 /* Rows back out of the pages, as the values the cache stands for: position start[b] + i of session b -> row cu[b] + i of k_out / v_out
- * (row type, row stride o_rs; either may be NULL).  Positions without a page read as zero. */
+ * (row type, row stride o_rs; either may be NULL).  Positions without a page read as zero; a session whose start is outside 0 .. 2^30 is left out. */
 int32_t s2s_op_kv_read_paged(void* stream, const s2s_paged_kv* kv, const int32_t* table_dev, int32_t table_cols, const int32_t* start_dev,
                              const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, void* k_out, void* v_out, int64_t o_rs);
 
 /* o = softmax(scale q k^T) v over the pages, H query heads in H / kv_heads neighbours per KV head.  kv_len_dev int32 [B]: positions in the cache,
  * the new rows' own among them.  causal: new row i of n sees the positions below kv_len - n + i + 1, window > 0 (causal only): the last
  * `window` of those.  A row that sees nothing is zero.  Pages may hold anything (NaN too) at positions at and behind kv_len; positions below it that
- * some row of the call sees hold numbers.  Scores, softmax and sums are f32.  scale: any number whose product with log2 e is finite, zero and negative ones too.
+ * some row of the call sees hold finite numbers (a value that is none also reaches rows it is hidden from).  Scores, softmax and sums are f32; the weights are
+ * operands of the second product: f32; bf16 twice (16 bits) where max_new H / kv_heads <= 16, or <= 64 with fewer than 64 (session, KV head) pairs, else bf16
+ * once; float16 over 4 bits.  A row's last bits so depend on the sizes of its call.  scale: any number whose product with log2 e is finite, zero and negative ones too.
  * ws_dev: s2s_op_attn_paged_ws(...) bytes (0: none needed), overwritten; calls that may run at the same time need one each. */
 int32_t s2s_op_attn_paged(void* stream, const s2s_paged_kv* kv, const void* q, int64_t q_rs, void* o, int64_t o_rs, int32_t H, const int32_t* table_dev,
                           int32_t table_cols, const int32_t* kv_len_dev, const int32_t* cu_dev, int32_t B, int32_t T, int32_t max_new, int32_t max_kv,

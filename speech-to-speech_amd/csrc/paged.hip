@@ -341,7 +341,7 @@ __device__ __forceinline__ void put_key(const AppendParams& p, int page, int h, 
 
 // One new row per session (a decode step): D / 8 lanes per row of a head, tasks = KV heads' keys, their values, query heads.  Bound by latency and by
 // the values' scattered columns (one element, or one nibble, per channel: 64-byte sectors of the transposed page).  64 sessions of 16 / 8 heads of 128, bf16:
-// 4.3 us; 512 sessions in 4 bits: 14.4 us, of which the sectors of the value columns (17 MB read, 17 MB written back) are half.
+// 4.3 us; 512 sessions in 4 bits: 14.0 us, of which the sectors of the value columns (17 MB read, 17 MB written back) are half.
 template <typename T, int KIND, int D, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendParams p) {
     constexpr int LPT = D / 8;
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(256) void kv_append_step_kernel(AppendParams p) {
 
 // Rows of a prompt: a workgroup takes the new rows that fall into one run of 64 positions (always inside one page) of: one KV head's keys; 64
 // channels of one KV head's values, transposed through LDS so that every channel's positions are written as whole octets; or a query head.  HBM-bound: 25 k rows of
-// 16 / 8 heads of 128, bf16: 97 us, 4.5 TB/s; in 4 bits 83 us, 4.2 TB/s (the divisions of the codes are 4 us of it).
+// 16 / 8 heads of 128, bf16: 97 us, 4.5 TB/s; in 4 bits 91 us, 3.8 TB/s (the divisions of the codes are 4 us of it).
 template <typename T, int KIND, int D, bool VEC>
 __global__ __launch_bounds__(256) void kv_append_block_kernel(AppendParams p) {
     constexpr int LD = sizeof(T) == 2 ? 66 : 65;      // 33 / 65 dwords per row: the column reads of 8 octets hit 4 or more different banks

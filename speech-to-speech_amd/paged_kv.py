@@ -218,7 +218,7 @@ class PagedKVCache:
 
     def read(self, table, start, cu=None, rows=None, *, max_new=None):
         """Positions ``start[b] + i`` of every session, back as rows (keys, values) [rows][kv_heads][head_dim] of the model type: what the cache stands for.
-        ``rows`` = cu[-1] where ``cu`` is given."""
+        ``rows`` = cu[-1] where ``cu`` is given.  Rows that are left out (behind cu[-1], beyond ``max_new``) hold anything."""
         if rows is None:
             _require(cu is None, "rows: how many rows cu counts")
             rows = table.shape[0]
@@ -239,8 +239,9 @@ class PagedKVCache:
     def attend(self, q, table, kv_len, cu=None, *, max_new=None, max_kv=None, scale=None, causal: bool = True, window: int = 0, out=None, workspace=None):
         """softmax(scale q k^T) v over the first ``kv_len[b]`` positions of every session (the new rows' own among them) -> ``out`` (new, or given).
         ``q`` [rows][heads][head_dim], heads a multiple of ``kv_heads``; ``scale`` (any finite number) None: head_dim ** -0.5.  causal: new row i of n sees the positions
-        below kv_len - n + i + 1, ``window`` > 0: the last ``window`` of those.  A row that sees nothing is zero.  ``workspace``: uint8 tensor of
-        ``workspace_bytes`` (None: taken from torch's allocator; one given to calls on several streams at once would be overwritten)."""
+        below kv_len - n + i + 1, ``window`` > 0: the last ``window`` of those.  A row that sees nothing is zero; rows that are left out stay as they
+        are in ``out`` and hold anything in a new one.  Keys and values that some row sees are finite.  ``workspace``: uint8 tensor of ``workspace_bytes`` (None: taken
+        from torch's allocator; one given to calls on several streams at once would be overwritten)."""
         device, dim = self.device, self.head_dim
         T, H, q_rs = _rows(q, None, dim, self.dtype, device, "q")
         b, cols, rows, max_new = self._sessions(table, kv_len, cu, T, max_new, "kv_len")
