@@ -260,8 +260,9 @@ int32_t s2s_op_attention(void* stream, const void* q, int64_t q_rs, const void* 
  * stored, its positions are not attended to.  A page that is written must belong to one session only; pages that are only read may be shared.
  * cu_dev int32 [B + 1]: session b's new rows are cu[b] .. cu[b + 1] - 1 of the row buffers (T rows); NULL: one row per session (T = B).
  * max_new: host-side bound of every session's new rows; max_kv: of every kv_len.  Buffers are read with row strides *_rs in elements, the
- * heads of a row lie next to each other; rows that are written share no memory, nor with rows that are read unless they are the same.  Rows at and behind cu[B] are left as they are.  Of a session beyond the bounds, or behind row T, the rows beyond are
- * not computed and the positions beyond not attended to; the others keep their places (n and kv_len below are the uncut numbers). */
+ * heads of a row lie next to each other; rows that are written share no memory with each other, nor with rows that are read unless they are those rows.
+ * Rows at and behind cu[B] are left as they are.  Of a session beyond the bounds, or behind row T, the rows beyond are not computed and the positions beyond
+ * not attended to; the others keep their places (n and kv_len below are the uncut numbers). */
 #define S2S_KV_MODEL 0
 #define S2S_KV_INT4 1
 typedef struct s2s_paged_kv {

@@ -253,3 +253,50 @@ def test_an_infinite_score_is_nan_where_it_is_seen_and_nothing_elsewhere(kind, d
     for o in outs:
         n = new if o is outs[0] else blind
         assert ((o[:n].double() - want[:n]).abs() <= tol[:n]).all()
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+@pytest.mark.parametrize("new,kv", [([1, 1, 1], [203, 64, 0]), ([1, 1], [4000, 3]), ([40, 0, 65], [40, 9, 300]), ([130, 7], [129, 3]), ([90], [3000])])
+def test_results_in_place_of_their_queries(kind, dtype, new, kv):
+    Hkv, H, D, B = 2, 4, 128, len(new)
+    table, n_pages = make_table(kv, 64, 0, 1)
+    cache, tb, lens, cu = poisoned(n_pages, Hkv, D, 64, kind, dtype), table.to(DEV), i32(kv), i32(ragged(new))
+    cache.append(randn(sum(kv), Hkv, D, seed=1, dtype=dtype).to(DEV), randn(sum(kv), Hkv, D, seed=2, dtype=dtype).to(DEV), tb, i32([0] * B), i32(ragged(kv)), max_new=max(kv))
+    q = randn(sum(new), H, D, seed=3, dtype=dtype).to(DEV)
+    want = cache.attend(q, tb, lens, cu, max_new=max(new), max_kv=max(kv))
+    assert cache.attend(q, tb, lens, cu, max_new=max(new), max_kv=max(kv), out=q) is q
+    assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("kind,dtype", KINDS)
+def test_a_captured_prompt_replays_beyond_its_bounds(kind, dtype):
+    """Lengths on the device pass the bounds of the capture and come back: every replay against the eager call, rows beyond left alone."""
+    Hkv, H, D, kvs = 2, 4, 64, [700, 3000]
+    table, n_pages = make_table(kvs, 64, 0, 1)
+    cache, tb = poisoned(n_pages, Hkv, D, 64, kind, dtype), table.to(DEV)
+    cache.append(randn(sum(kvs), Hkv, D, seed=1, dtype=dtype).to(DEV), randn(sum(kvs), Hkv, D, seed=2, dtype=dtype).to(DEV), tb, i32([0, 0]), i32(ragged(kvs)), max_new=max(kvs))
+    q, lens, cu = torch.zeros(200, H, D, dtype=dtype, device=DEV), i32([600, 2500]), i32([0, 50, 130])
+    args, out = dict(max_new=80, max_kv=2600), torch.zeros_like(q)
+    ws = torch.zeros(max(16, cache.workspace_bytes(H, 2, 200, **args)), dtype=torch.uint8, device=DEV)
+    cache.attend(q, tb, lens, cu, out=out, workspace=ws, **args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        cache.attend(q, tb, lens, cu, out=out, workspace=ws, **args)
+    for i, (kv, new) in enumerate((([600, 2500], [50, 80]), ([700, 3000], [120, 80]), ([700, 2600], [20, 170]), ([90, 2601], [80, 81]), ([600, 2500], [50, 80]))):
+        q.copy_(randn(200, H, D, seed=10 + i, dtype=dtype))
+        lens.copy_(i32(kv))
+        cu.copy_(i32(ragged(new)))
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = torch.full_like(out, 3.0)
+        cache.attend(q, tb, lens, cu, out=want, **args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        at = 0
+        for n in new:
+            assert (out[at : at + min(n, 80)] != 3).any(-1).all() and (out[at + min(n, 80) : at + n] == 3).all()
+            at += n
+        assert (out[at:] == 3).all()
